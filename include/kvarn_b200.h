@@ -76,7 +76,7 @@ typedef struct kvb_layer {
 } kvb_layer;
 
 /* bits OR-ed into *error_word */
-enum { KVB_ERR_PAGE_RANGE = 1u, KVB_ERR_TABLE_RANGE = 2u, KVB_ERR_WAIT_TIMEOUT = 4u, KVB_ERR_POSITIONS = 8u, KVB_ERR_GEOMETRY = 16u };
+enum { KVB_ERR_PAGE_RANGE = 1u, KVB_ERR_TABLE_RANGE = 2u, KVB_ERR_WAIT_TIMEOUT = 4u, KVB_ERR_POSITIONS = 8u, KVB_ERR_GEOMETRY = 16u, KVB_ERR_SLOT = 32u };
 
 const char* kvb_last_error_string(void);
 int kvb_version(void);
@@ -251,6 +251,76 @@ size_t kvb_prefill_workspace_bytes(int kv_len_max, int kv_heads, int q_heads, in
  * (P3:3508-3610, 2362-2416), the merge it feeds repeats their split reduction (P3:3149-3170, 3467-3482). */
 int kvb_attn_chunk_partial(const kvb_layer* layer, const void* q, const int32_t* positions_dev, int tokens, float scale,
                            int kv_len_max, void* workspace, float* part_m, float* part_l, float* part_o, void* stream);
+
+/* ---- Rotary positions.  No counterpart in the reference, whose cache takes rows that its engine has turned already. ----
+ * Dims (i, j) of pair p of a head at position t become  x_i c - x_j s, x_j c + x_i s  with  c + i s = factor * exp(i t inv_freq[p]);
+ * (i, j) = (p, p + rotary_dim / 2), or (2 p, 2 p + 1) where `interleaved` is 1; dims from rotary_dim on pass.  Computed in fp32 from angles
+ * reduced in 64 bits: any int32 position. */
+typedef struct kvb_rope {
+    const double* inv_freq; /* device: rotary_dim / 2 angles (radians) per position */
+    float factor;           /* of cosine and sine; 1, or the attention factor of a scaled context */
+    int32_t rotary_dim;     /* even, 2..head_dim */
+    int32_t interleaved;    /* 0 or 1 */
+} kvb_rope;
+
+/* Frequencies into HOST memory: inv_freq[rotary_dim / 2] and the factor that goes with them.
+ *   KVB_ROPE_PLAIN   base^(-2 p / rotary_dim)
+ *   KVB_ROPE_LINEAR  those / factor (position interpolation)
+ *   KVB_ROPE_NTK     base * factor^(rotary_dim / (rotary_dim - 2)) as the base
+ *   KVB_ROPE_YARN    by parts: pairs of more than 32 turns over original_len positions as they are, those of less than one / factor, a ramp between
+ *                    (over whole pairs), and 0.1 ln(factor) + 1 as the attention factor */
+enum { KVB_ROPE_PLAIN = 0, KVB_ROPE_LINEAR = 1, KVB_ROPE_NTK = 2, KVB_ROPE_YARN = 3 };
+int kvb_rope_frequencies(int rotary_dim, double base, int scaling, double factor, int original_len, double* inv_freq, float* attention_factor);
+
+/* Turn rows: x, out [tokens][heads][head_dim] of `dtype`, tokens *_stride elements apart (heads * head_dim where rows are packed; more where they
+ * are part of a wider buffer, e.g. the queries and keys of a fused projection).  positions_dev[tokens]: any positions.  out may be x itself (same
+ * stride), or rows beside those of x in one buffer; other shared memory is refused.  Fast (16 bytes an access) where rows and strides keep to
+ * 16 bytes and rotary_dim is a multiple of 16 (interleaved: 8). */
+int kvb_rope_rows(const kvb_rope* rope, const void* x, int64_t x_stride, void* out, int64_t out_stride, const int32_t* positions_dev, int tokens, int heads,
+                  int head_dim, int dtype, void* stream);
+
+/* kvb_append of keys that are turned on the way, and (q not NULL) queries turned beside it into q_out, in one launch.  Keys go from the turn into
+ * the cache's own rotation in fp32, without the rounding to `dtype` that kvb_rope_rows followed by kvb_append makes.  q, q_out:
+ * [tokens][q_heads][head_dim]; k, v: [tokens][kv_heads][head_dim]; strides in elements from token to token.  q_out may be q itself; it shares no
+ * other memory with q, k, v or the positions.  Positions that are not contiguous set KVB_ERR_POSITIONS, and the call leaves cache and q_out alone. */
+int kvb_rope_append(const kvb_layer* layer, const kvb_rope* rope, const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride, const void* k, int64_t k_stride,
+                    const void* v, int64_t v_stride, const int32_t* positions_dev, int tokens, void* stream);
+
+/* Rows [begin, begin + tokens) of the cache as keys and values again: de-quantised (rows of the open tile: from the stage) and turned back out of the
+ * Walsh-Hadamard domain, [tokens][kv_heads][head_dim] of the layer's dtype; 16-byte aligned outputs.  *total_pos_dev: position of the newest token,
+ * which tells the open tile; rows behind it, and rows of a tile with a bad page (error word), are left as they are.  Positions stay in
+ * the keys.  For handing a prefix on, or comparing; the reference keeps such rows in its bf16 mirror (LAUNCH.h:70-91). */
+int kvb_read_rows(const kvb_layer* layer, int begin, int tokens, const int32_t* total_pos_dev, void* out_k, void* out_v, void* stream);
+
+/* ---- Linear attention with a decay for each head: the layers of a hybrid model that keep a state instead of a cache.  No counterpart in the reference. ----
+ *   S_t = exp(log_decay[head]) S_{t-1} + k_t v_t^T,   o_t = scale * q_t S_t
+ * per sequence and value head; S: [head_dim of k][head_dim of v], fp32.  Value head h goes with query and key head h / (v_heads / qk_heads). */
+typedef struct kvb_linear {
+    float* state;           /* [slots][v_heads][head_dim][head_dim], 16-byte aligned; a new sequence starts from zeros */
+    const float* log_decay; /* device [v_heads], natural logarithm, <= 0 (-infinity: nothing is kept); a head with another one sets
+                               KVB_ERR_GEOMETRY and is left alone */
+    int32_t slots;
+    int32_t qk_heads, v_heads; /* v_heads a multiple of qk_heads, at most 256 */
+    int32_t head_dim;          /* 64 or 128 */
+    int32_t dtype;             /* KVB_DTYPE_* of q, k, v and out */
+    uint32_t* error_word;      /* optional device word */
+} kvb_linear;
+
+/* One token of each of `batch` (0..256) sequences.  q, k: [batch][qk_heads][head_dim], v: [batch][v_heads][head_dim], strides in elements from row to
+ * row; out: [batch][v_heads][head_dim], packed, in memory of its own.  The state of sequence b is read from slot reads_dev[b] and written to slot
+ * writes_dev[b]: the same one for a step in place; another one where the old state is still wanted (drafts that may be rolled back), and several
+ * sequences may read one slot (a shared prefix).  A sequence whose slot is out of range, that writes a slot which another one of the call
+ * reads or writes, or reads one which another writes, sets KVB_ERR_SLOT and is left alone. */
+int kvb_linear_decode(const kvb_linear* layer, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride, int batch,
+                      const int32_t* reads_dev, const int32_t* writes_dev, float scale, void* out, void* stream);
+
+/* The same over several tokens of each sequence, packed one sequence behind another: rows offsets_dev[b] .. offsets_dev[b + 1] - 1 belong to sequence
+ * b (offsets_dev[batch + 1], not falling, within 0..tokens; a sequence without rows has its state copied).  Rows outside all sequences are left as they are.
+ * Offsets that fall or leave the rows set KVB_ERR_POSITIONS; that sequence is left alone.  workspace: kvb_linear_workspace_bytes(tokens, batch, ...) bytes. */
+size_t kvb_linear_workspace_bytes(int tokens, int batch, int v_heads, int head_dim);
+int kvb_linear_chunk(const kvb_linear* layer, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                     const int32_t* offsets_dev, int batch, int tokens, const int32_t* reads_dev, const int32_t* writes_dev, float scale, void* workspace, void* out,
+                     void* stream);
 
 #ifdef __cplusplus
 }

@@ -23,4 +23,9 @@ def __getattr__(name):
 
         cache = importlib.import_module(__name__ + ".cache")
         return cache if name == "cache" else getattr(cache, name)
+    if name in ("Rope", "LinearAttention", "rope", "linear"):
+        import importlib
+
+        mod = importlib.import_module(__name__ + (".rope" if name in ("Rope", "rope") else ".linear"))
+        return mod if name in ("rope", "linear") else getattr(mod, name)
     raise AttributeError(name)

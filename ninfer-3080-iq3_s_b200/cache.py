@@ -25,6 +25,21 @@ def _stream():
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
+def row_stride(x: torch.Tensor, heads: int, head_dim: int, dtype: torch.dtype, tokens: int | None = None) -> int:
+    """Elements from token to token of rows [tokens, heads, head_dim] whose heads are packed; anything else is refused."""
+    if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != head_dim or x.dtype != dtype or (tokens is not None and x.shape[0] != tokens):
+        raise ValueError(f"rows [{'tokens' if tokens is None else tokens}, {heads}, {head_dim}] of {dtype}: got {tuple(x.shape)} of {x.dtype}")
+    at = x.stride()
+    if at[2] != 1 or (heads > 1 and at[1] != head_dim):
+        raise ValueError(f"the heads of a token lie packed: got strides {at}")
+    return at[0]
+
+
+def check_positions(positions: torch.Tensor, tokens: int) -> None:
+    if positions.dtype != torch.int32 or positions.shape != (tokens,) or not positions.is_contiguous():
+        raise ValueError(f"positions: int32 [{tokens}], got {tuple(positions.shape)} of {positions.dtype}")
+
+
 # Workspace sizes are functions of the shape (and of the device's SM count): a step asks for the same one in every layer.
 @functools.lru_cache(maxsize=256)
 def _workspace_bytes(device, kv_len_max, kv_heads, q_heads, head_dim, rows):
@@ -73,6 +88,33 @@ class KvarnLayer:
     def append(self, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor) -> None:
         """k, v: [tokens, kv_heads, head_dim]; positions: int32 [tokens] on the device, contiguous."""
         capi.check(capi.load().kvb_append(C.byref(self.c), _ptr(k), _ptr(v), _ptr(positions), int(k.shape[0]), _stream()))
+
+    # ---- the same with keys (and queries, beside it) turned by their positions; no counterpart in the reference
+    def rope_append(self, rope, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, q: torch.Tensor | None = None, q_out: torch.Tensor | None = None):
+        """k, v: [tokens, kv_heads, head_dim], q: [tokens, q_heads, head_dim], rows packed or parts of wider ones; `rope`: a rope.Rope.
+        Returns the turned queries (None without q)."""
+        tokens, (kv, qh, d) = int(k.shape[0]), (self.kv_heads, self.q_heads, self.head_dim)
+        ks, vs = row_stride(k, kv, d, self.dtype, tokens), row_stride(v, kv, d, self.dtype, tokens)
+        check_positions(positions, tokens)
+        qs = os = 0
+        if q is not None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+            qs, os = row_stride(q, qh, d, self.dtype, tokens), row_stride(q_out, qh, d, self.dtype, tokens)
+        capi.check(capi.load().kvb_rope_append(C.byref(self.c), C.byref(rope.c), _ptr(q), qs, _ptr(q_out), os, _ptr(k), ks, _ptr(v), vs, _ptr(positions),
+                                               tokens, _stream()))
+        return q_out
+
+    # ---- rows back as keys and values (the reference: its bf16 mirror, kvarn128_window*)
+    def read_rows(self, begin: int, tokens: int, pos: torch.Tensor, out_k: torch.Tensor | None = None, out_v: torch.Tensor | None = None):
+        """Rows [begin, begin + tokens) as [tokens, kv_heads, head_dim]; pos: int32 [1] on the device, the newest token's position."""
+        check_positions(pos, 1)
+        shape = (tokens, self.kv_heads, self.head_dim)
+        out_k, out_v = (torch.empty(shape, dtype=self.dtype, device=self.device) if x is None else x for x in (out_k, out_v))
+        for x in (out_k, out_v):
+            if x.shape != shape or x.dtype != self.dtype or not x.is_contiguous():
+                raise ValueError(f"outputs: packed rows {list(shape)} of {self.dtype}")
+        capi.check(capi.load().kvb_read_rows(C.byref(self.c), begin, tokens, _ptr(pos), _ptr(out_k), _ptr(out_v), _stream()))
+        return out_k, out_v
 
     # ---- kvarn128_decode_tile
     def decode_tile(self, tile: int, head: int):

@@ -13,7 +13,8 @@ LIB_PATH = os.environ.get("KVB_LIBRARY", os.path.join(_HERE, "libkvarn_b200.so")
 
 KVB_OK, KVB_EINVAL, KVB_ECUDA, KVB_ERANGE, KVB_ETIMEOUT = range(5)
 DTYPE_F16, DTYPE_BF16 = 0, 1
-ERR_PAGE_RANGE, ERR_TABLE_RANGE, ERR_WAIT_TIMEOUT, ERR_POSITIONS, ERR_GEOMETRY = 1, 2, 4, 8, 16
+ERR_PAGE_RANGE, ERR_TABLE_RANGE, ERR_WAIT_TIMEOUT, ERR_POSITIONS, ERR_GEOMETRY, ERR_SLOT = 1, 2, 4, 8, 16, 32
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_YARN = range(4)
 
 
 class KvarnError(RuntimeError):
@@ -35,6 +36,15 @@ class kvb_layer(C.Structure):
 class kvb_peer_ring(C.Structure):
     _fields_ = [("peer_bufs", C.POINTER(C.c_void_p)), ("local_buf", C.c_void_p), ("state", C.c_void_p), ("rank", C.c_int32),
                 ("world", C.c_int32), ("max_spins", C.c_uint32), ("rows", C.c_uint32)]
+
+
+class kvb_rope(C.Structure):
+    _fields_ = [("inv_freq", C.c_void_p), ("factor", C.c_float), ("rotary_dim", C.c_int32), ("interleaved", C.c_int32)]
+
+
+class kvb_linear(C.Structure):
+    _fields_ = [("state", C.c_void_p), ("log_decay", C.c_void_p), ("slots", C.c_int32), ("qk_heads", C.c_int32), ("v_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("dtype", C.c_int32), ("error_word", C.c_void_p)]
 
 
 # name -> (restype, argtypes); every symbol the header declares
@@ -78,6 +88,17 @@ SYMBOLS = {
     "kvb_prefill_workspace_bytes": (C.c_size_t, [C.c_int] * 5),
     "kvb_attn_chunk_partial": (C.c_int, [C.POINTER(kvb_layer), C.c_void_p, C.c_void_p, C.c_int, C.c_float, C.c_int, C.c_void_p,
                                          C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "kvb_rope_frequencies": (C.c_int, [C.c_int, C.c_double, C.c_int, C.c_double, C.c_int, C.POINTER(C.c_double), C.POINTER(C.c_float)]),
+    "kvb_rope_rows": (C.c_int, [C.POINTER(kvb_rope), C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int,
+                                C.c_void_p]),
+    "kvb_rope_append": (C.c_int, [C.POINTER(kvb_layer), C.POINTER(kvb_rope), C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                  C.c_void_p, C.c_int64, C.c_void_p, C.c_int, C.c_void_p]),
+    "kvb_read_rows": (C.c_int, [C.POINTER(kvb_layer), C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "kvb_linear_decode": (C.c_int, [C.POINTER(kvb_linear), C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int, C.c_void_p,
+                                    C.c_void_p, C.c_float, C.c_void_p, C.c_void_p]),
+    "kvb_linear_workspace_bytes": (C.c_size_t, [C.c_int] * 4),
+    "kvb_linear_chunk": (C.c_int, [C.POINTER(kvb_linear), C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int,
+                                   C.c_int, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p]),
 }
 
 _lib = None

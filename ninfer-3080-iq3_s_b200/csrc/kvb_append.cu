@@ -12,6 +12,9 @@
 //   scale_axis = fp16(best_row * scale);  zp_axis = fp16(best_row * lo);  other_axis = fp16(best_col)
 #include "kvb_common.cuh"
 #include "kvb_ptx.cuh"
+#include "kvb_rope.cuh"
+
+#include <type_traits>
 
 namespace kvb {
 namespace {
@@ -299,15 +302,47 @@ __device__ void quantize_slice(AppendSmem& sm, float (&x)[kPer]) {
     __syncthreads();
 }
 
+// What happens to a row between global memory and its Walsh-Hadamard rotation: nothing, or the turn of its position.
+struct NoTurn {
+    static constexpr bool kTurns = false;
+    __device__ __forceinline__ void ready() const {}
+};
+// The angles of a tile's new rows meet in shared memory, [row][pair], each computed once for the CTA's head; that runs while the rows are
+// under way from global memory.  Rows of fp32 go on to the Walsh-Hadamard rotation: nothing is rounded in between.
+struct RopeTurn {
+    static constexpr bool kTurns = true;
+    RopeView rope;
+    float2* table;
+    int stride;  // entries from row to row: an odd number of 16-byte words more than the pairs, so that rows fall on different banks
+    int first, rows;  // position of the tile's first new row, and their number
+    __device__ __forceinline__ void ready() const {
+        const int pairs = rope.rotary / 2;
+        for (int i = threadIdx.x; i < rows * pairs; i += kThreads) {
+            const int r = i / pairs, p = i - r * pairs;
+            table[r * stride + p] = rope_turn(rope.inv_freq[p], first + r, rope.factor);
+        }
+        __syncthreads();
+    }
+    // dim d's other half, its pair, and whether d is the pair's first
+    __device__ __forceinline__ int peer(int d) const { return rope.interleaved ? d ^ 1 : d < rope.rotary / 2 ? d + rope.rotary / 2 : d - rope.rotary / 2; }
+    __device__ __forceinline__ int pair(int d) const { return rope.interleaved ? d >> 1 : d < rope.rotary / 2 ? d : d - rope.rotary / 2; }
+    __device__ __forceinline__ bool is_first(int d) const { return rope.interleaved ? (d & 1) == 0 : d < rope.rotary / 2; }
+    __device__ __forceinline__ float turned(int row, int d, float x, float other) const {
+        const float2 t = table[row * stride + pair(d)];
+        return is_first(d) ? turn_first(x, other, t) : turn_second(x, other, t);
+    }
+};
+__host__ __device__ constexpr int rope_table_stride(int rotary) { return (rotary / 2 + 1) / 2 * 2 + 2; }
+
 // The new rows begin .. end - 1 of tile `base`, rotated (stages, order and roundings of hadamard_warp).  A lane holds 32 neighbouring
 // dims of a row: D / 32 lanes a row, 1024 / D rows a warp at a time; the strides up to 16 stay inside a lane, in pairs of dims, those of
 // 32 and more cross lanes, and rows are read and stored 16 bytes at a time.  A warp has up to 8 rows of the tile and reads them all before
 // rotating any: it waits for global memory once.  `keep(row, d, x)` takes dims d .. d + 7 of the slice.  Measured on B200 against a
 // warp a row with dims l + 32 r in lane l (five strides by shuffles, two bytes an access) and a division a code, us a call, graph replay of 1,024
 // tokens: 128 dims 9.9 -> 7.0, 256 dims 12.5 -> 9.3; calls in a row: with 16 rounds of balancing 31.8 -> 27.1, a prompt of 777 tokens 32.6 -> 29.2.
-// The rows start at 16-byte boundaries.
-template <int D, bool kBf16, typename Keep>
-__device__ __forceinline__ void rotate_rows(const uint16_t* __restrict__ src, int64_t row_stride, int begin, int end, int slice, Keep keep) {
+// The rows start at 16-byte boundaries; where they are turned, the turning part has whole groups of 8 dims in either half.
+template <int D, bool kBf16, typename Keep, typename Turn>
+__device__ __forceinline__ void rotate_rows(const uint16_t* __restrict__ src, int64_t row_stride, int begin, int end, int slice, Keep keep, const Turn& turn) {
     constexpr int kLanes = D / 32, kAtOnce = 32 / kLanes, kWarpsPerCta = kThreads / 32, kPasses = kTile / (kWarpsPerCta * kAtOnce);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, block = lane % kLanes;
     uint4 raw[kPasses][4];
@@ -318,6 +353,20 @@ __device__ __forceinline__ void rotate_rows(const uint16_t* __restrict__ src, in
 #pragma unroll
         for (int c = 0; c < 4; ++c) raw[u][c] = tt >= end ? make_uint4(0u, 0u, 0u, 0u) : reinterpret_cast<const uint4*>(row)[c];
     }
+    uint4 other[Turn::kTurns ? kPasses : 1][4];  // the other halves of the same pairs
+    if constexpr (Turn::kTurns) {
+#pragma unroll
+        for (int u = 0; u < kPasses; ++u) {
+            const int tt = begin + warp + kWarpsPerCta * (u * kAtOnce + lane / kLanes);
+            const uint16_t* row = src + (tt - begin) * row_stride;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int d = 32 * block + 8 * c;
+                other[u][c] = tt < end && d < turn.rope.rotary && !turn.rope.interleaved ? *reinterpret_cast<const uint4*>(row + turn.peer(d)) : make_uint4(0u, 0u, 0u, 0u);
+            }
+        }
+    }
+    turn.ready();
 #pragma unroll
     for (int u = 0; u < kPasses; ++u) {
         if (begin + warp + kWarpsPerCta * u * kAtOnce >= end) break;  // no row left for any lane
@@ -325,12 +374,37 @@ __device__ __forceinline__ void rotate_rows(const uint16_t* __restrict__ src, in
         F2 x[16];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            const uint32_t w[4] = {raw[u][c].x, raw[u][c].y, raw[u][c].z, raw[u][c].w};
+            float y[8];
+            unpack8_16<kBf16>(raw[u][c], y);
+            if constexpr (Turn::kTurns) {
+                const int d = 32 * block + 8 * c;
+                if (d < turn.rope.rotary && tt < end) {
+                    const float4* t = reinterpret_cast<const float4*>(turn.table + (tt - begin) * turn.stride + turn.pair(d));
+                    if (turn.rope.interleaved) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {  // the stride of 1 lies inside a pair
-                const float lo = in_to_f32<kBf16>(static_cast<uint16_t>(w[e])), hi = in_to_f32<kBf16>(static_cast<uint16_t>(w[e] >> 16));
-                x[4 * c + e] = F2(__fadd_rn(lo, hi), __fsub_rn(lo, hi));
+                        for (int e = 0; e < 2; ++e) {
+                            const float4 a = t[e];
+                            const float y0 = y[4 * e], y1 = y[4 * e + 1], y2 = y[4 * e + 2], y3 = y[4 * e + 3];
+                            y[4 * e] = turn_first(y0, y1, make_float2(a.x, a.y));
+                            y[4 * e + 1] = turn_second(y1, y0, make_float2(a.x, a.y));
+                            y[4 * e + 2] = turn_first(y2, y3, make_float2(a.z, a.w));
+                            y[4 * e + 3] = turn_second(y3, y2, make_float2(a.z, a.w));
+                        }
+                    } else {
+                        float z[8];
+                        unpack8_16<kBf16>(other[u][c], z);
+                        const float sign = turn.is_first(d) ? -1.0f : 1.0f;  // exact, so both halves are one formula
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float4 a = t[e];
+                            y[2 * e] = turn_second(y[2 * e], z[2 * e], make_float2(a.x, __fmul_rn(a.y, sign)));
+                            y[2 * e + 1] = turn_second(y[2 * e + 1], z[2 * e + 1], make_float2(a.z, __fmul_rn(a.w, sign)));
+                        }
+                    }
+                }
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * c + e] = F2(__fadd_rn(y[2 * e], y[2 * e + 1]), __fsub_rn(y[2 * e], y[2 * e + 1]));  // the stride of 1 lies inside a pair
         }
 #pragma unroll
         for (int span = 1; span <= 8; span <<= 1)
@@ -369,8 +443,8 @@ __device__ __forceinline__ void rotate_rows(const uint16_t* __restrict__ src, in
 
 // The same, a warp a row with dims l + 32 r in lane l: from any 2-byte boundary, up to 16 kBatch rows.  `keep(row, d, h)` takes dim d of the
 // slice.
-template <int D, bool kBf16, int kBatch, typename Keep>
-__device__ __forceinline__ void rotate_rows_singly(const uint16_t* __restrict__ src, int64_t row_stride, int begin, int end, int slice, Keep keep) {
+template <int D, bool kBf16, int kBatch, typename Keep, typename Turn>
+__device__ __forceinline__ void rotate_rows_singly(const uint16_t* __restrict__ src, int64_t row_stride, int begin, int end, int slice, Keep keep, const Turn& turn) {
     constexpr int kWarpsPerCta = kThreads / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint16_t raw[kBatch][D / 32];
@@ -383,13 +457,38 @@ __device__ __forceinline__ void rotate_rows_singly(const uint16_t* __restrict__ 
             for (int r = 0; r < D / 32; ++r) raw[u][r] = row[lane + 32 * r];
         }
     }
+    // the other halves of the pairs: asked for beside the rows where there are few of them, else as they are needed, out of the L1
+    constexpr bool kAhead = Turn::kTurns && kBatch <= 3;
+    uint16_t other[kAhead ? kBatch : 1][D / 32];
+    if constexpr (kAhead) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int tt = begin + warp + u * kWarpsPerCta;
+            if (tt < end) {
+                const uint16_t* row = src + (tt - begin) * row_stride;
+#pragma unroll
+                for (int r = 0; r < D / 32; ++r)
+                    if (lane + 32 * r < turn.rope.rotary) other[u][r] = row[turn.peer(lane + 32 * r)];
+            }
+        }
+    }
+    turn.ready();
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
         const int tt = begin + warp + u * kWarpsPerCta;
         if (tt >= end) break;
         float val[D / 32];
 #pragma unroll
-        for (int r = 0; r < D / 32; ++r) val[r] = in_to_f32<kBf16>(raw[u][r]);
+        for (int r = 0; r < D / 32; ++r) {
+            val[r] = in_to_f32<kBf16>(raw[u][r]);
+            if constexpr (Turn::kTurns) {
+                const int d = lane + 32 * r;
+                if (d < turn.rope.rotary) {
+                    const uint16_t z = kAhead ? other[kAhead ? u : 0][r] : src[(tt - begin) * row_stride + turn.peer(d)];
+                    val[r] = turn.turned(tt - begin, d, val[r], in_to_f32<kBf16>(z));
+                }
+            }
+        }
         hadamard_warp<D>(val, lane);
 #pragma unroll
         for (int r = 0; r < 4; ++r) keep(tt, lane + 32 * r, __float2half_rn(D == 128 || slice == 0 ? val[r] : val[D / 32 - 4 + r]));
@@ -414,10 +513,20 @@ template <int D> __device__ __forceinline__ bool rotates_singly(int rows, bool w
 // re-opens it.  Earlier tiles of a long append would be overwritten within the same call anyway.  When the first tile
 // begins inside (its earlier rows are read from the stage) and one of the last two, a different one, has the same slot, the
 // first tile's CTA writes that tile's rows too, after it has read its own: no second launch, no order between CTAs.
-template <int D, bool kBf16>
+//
+// With kRope, K rows are turned by their positions on the way, and the grid's columns from `tiles` on turn the query rows instead.
+struct AppendRope {
+    RopeView rope;
+    RopeRows q;    // q.x null: no queries
+    int64_t k_stride, v_stride;
+    int tiles, table_stride;
+    bool wide_k, wide_v, wide_q;
+};
+struct NoRope {};
+template <int D, bool kBf16, bool kRope>
 __global__ void __launch_bounds__(kThreads, 1) append_kernel(LayerView L, const uint16_t* __restrict__ k,
                                                              const uint16_t* __restrict__ v,
-                                                             const int32_t* __restrict__ positions, int tokens) {
+                                                             const int32_t* __restrict__ positions, int tokens, std::conditional_t<kRope, AppendRope, NoRope> R) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     AppendSmem& sm = *reinterpret_cast<AppendSmem*>(smem_raw);
     using G = Geo<D>;
@@ -428,6 +537,17 @@ __global__ void __launch_bounds__(kThreads, 1) append_kernel(LayerView L, const 
     if (pos0 < 0 || last - pos0 != tokens - 1) {  // positions must be contiguous and non-negative
         if (threadIdx.x == 0) L.flag(KVB_ERR_POSITIONS);
         return;
+    }
+    if constexpr (kRope) {
+        if (static_cast<int>(blockIdx.x) >= R.tiles) {
+            const int64_t ctas = static_cast<int64_t>(gridDim.x - R.tiles) * gridDim.y * gridDim.z;
+            const int64_t cta = (static_cast<int64_t>(blockIdx.x - R.tiles) * gridDim.y + blockIdx.y) * gridDim.z + blockIdx.z;
+            for (int64_t item = cta * kThreads + threadIdx.x; item < R.q.items; item += ctas * kThreads) {
+                if (R.wide_q) rope_item<kBf16, true>(R.q, item);
+                else rope_item<kBf16, false>(R.q, item);
+            }
+            return;
+        }
     }
     const AppendTile t = append_tile(pos0, last, blockIdx.x);
     if (!t.in_range) return;
@@ -446,9 +566,13 @@ __global__ void __launch_bounds__(kThreads, 1) append_kernel(LayerView L, const 
                 *reinterpret_cast<const uint4*>(src + static_cast<int64_t>(r) * D + c * 8);
         }
     }
-    const int64_t row_stride = static_cast<int64_t>(L.kv_heads) * D;
+    int64_t row_stride = static_cast<int64_t>(L.kv_heads) * D;
     const uint16_t* src = (which ? v : k) + static_cast<int64_t>(head) * D;
-    const bool wide = (reinterpret_cast<uintptr_t>(src) & 15u) == 0;
+    bool wide = (reinterpret_cast<uintptr_t>(src) & 15u) == 0;
+    if constexpr (kRope) {
+        row_stride = which ? R.v_stride : R.k_stride;
+        wide = which ? R.wide_v : R.wide_k;
+    }
     // the new rows of a tile into shared memory and its stage rows, 16 bytes or one element at a time
     auto rotate = [&](const AppendTile& a, bool here, bool to_stage) {
         const uint16_t* const rows = src + (a.base + a.begin - pos0) * row_stride;
@@ -458,9 +582,18 @@ __global__ void __launch_bounds__(kThreads, 1) append_kernel(LayerView L, const 
             if (here) *reinterpret_cast<X*>(&sm.rows[tt * kRowStride + d]) = x;
             if (to_stage) *reinterpret_cast<X*>(&stage[tt * D + d]) = x;
         };
-        if (rotates_singly<D>(a.end - a.begin, wide, L.iters > 0)) rotate_rows_singly<D, kBf16, 3>(rows, row_stride, a.begin, a.end, slice, keep);
-        else if (wide) rotate_rows<D, kBf16>(rows, row_stride, a.begin, a.end, slice, keep);
-        else rotate_rows_singly<D, kBf16, 8>(rows, row_stride, a.begin, a.end, slice, keep);
+        auto by_size = [&](const auto& turn) {
+            if (rotates_singly<D>(a.end - a.begin, wide, L.iters > 0)) rotate_rows_singly<D, kBf16, 3>(rows, row_stride, a.begin, a.end, slice, keep, turn);
+            else if (wide) rotate_rows<D, kBf16>(rows, row_stride, a.begin, a.end, slice, keep, turn);
+            else rotate_rows_singly<D, kBf16, 8>(rows, row_stride, a.begin, a.end, slice, keep, turn);
+        };
+        if constexpr (kRope) {
+            if (!which) {
+                by_size(RopeTurn{R.rope, reinterpret_cast<float2*>(smem_raw + sizeof(AppendSmem)), R.table_stride, a.base + a.begin, a.end - a.begin});
+                return;
+            }
+        }
+        by_size(NoTurn{});
     };
     rotate(t, true, write_stage);
     if (!seal) return;
@@ -562,10 +695,28 @@ int launch_append(const LayerView& V, const void* k, const void* v, const int32_
     static_assert(sizeof(AppendSmem) <= 227 * 1024, "shared memory");
     static OncePerDevice opted;  // per template instance
     const int smem = static_cast<int>(sizeof(AppendSmem));
-    KVB_CUDA_OK(allow_smem(opted, append_kernel<D, kBf16>, smem));
+    KVB_CUDA_OK(allow_smem(opted, append_kernel<D, kBf16, false>, smem));
     const dim3 grid(tokens / kTile + 2, V.kv_heads, 2 * Geo<D>::S);
-    KVB_CUDA_OK(launch_early(append_kernel<D, kBf16>, grid, dim3(kThreads), smem, stream, V, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
-                             positions, tokens));
+    KVB_CUDA_OK(launch_early(append_kernel<D, kBf16, false>, grid, dim3(kThreads), smem, stream, V, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
+                             positions, tokens, NoRope{}));
+    return KVB_OK;
+}
+
+template <int D, bool kBf16>
+int launch_rope_append(const LayerView& V, AppendRope R, const void* k, const void* v, const int32_t* positions, int tokens, cudaStream_t stream) {
+    static_assert(sizeof(AppendSmem) % 16 == 0 && sizeof(AppendSmem) + kTile * sizeof(float2) * rope_table_stride(D) <= 227 * 1024, "shared memory");
+    static OncePerDevice opted;  // per template instance
+    KVB_CUDA_OK(allow_smem(opted, append_kernel<D, kBf16, true>, static_cast<int>(sizeof(AppendSmem) + kTile * sizeof(float2) * rope_table_stride(D))));
+    R.tiles = tokens / kTile + 2;
+    R.table_stride = rope_table_stride(R.rope.rotary);
+    const int smem = static_cast<int>(sizeof(AppendSmem) + (tokens < kTile ? tokens : kTile) * sizeof(float2) * R.table_stride);
+    // the queries' items: a CTA's threads once over, in whole columns of the grid, on no more CTAs than the device has SMs
+    const int column = V.kv_heads * 2 * Geo<D>::S;
+    int64_t ctas = R.q.x == nullptr ? 0 : (R.q.items + kThreads - 1) / kThreads;
+    if (ctas > device_sm_count()) ctas = device_sm_count();
+    const dim3 grid(R.tiles + static_cast<unsigned>((ctas + column - 1) / column), V.kv_heads, 2 * Geo<D>::S);
+    KVB_CUDA_OK(launch_early(append_kernel<D, kBf16, true>, grid, dim3(kThreads), smem, stream, V, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
+                             positions, tokens, R));
     return KVB_OK;
 }
 
@@ -588,6 +739,47 @@ extern "C" int kvb_append(const kvb_layer* layer, const void* k, const void* v, 
                                           : launch_append<128, false>(V, k, v, positions_dev, tokens, s);
     return bf ? launch_append<256, true>(V, k, v, positions_dev, tokens, s)
               : launch_append<256, false>(V, k, v, positions_dev, tokens, s);
+}
+
+extern "C" int kvb_rope_append(const kvb_layer* layer, const kvb_rope* rope, const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride, const void* k,
+                               int64_t k_stride, const void* v, int64_t v_stride, const int32_t* positions_dev, int tokens, void* stream) {
+    using namespace kvb;
+    if (tokens == 0) return KVB_OK;
+    if (int st = check_layer(layer, "kvb_rope_append")) return st;
+    const int D = layer->head_dim;
+    if (int st = check_rope(rope, D, "kvb_rope_append")) return st;
+    if (tokens < 0) return fail(KVB_EINVAL, "kvb_rope_append: tokens = %d", tokens);
+    if (k == nullptr || v == nullptr || positions_dev == nullptr) return fail(KVB_EINVAL, "kvb_rope_append: null k / v / positions");
+    if ((q == nullptr) != (q_out == nullptr)) return fail(KVB_EINVAL, "kvb_rope_append: q and q_out come together");
+    if (layer->stage == nullptr) return fail(KVB_EINVAL, "kvb_rope_append: layer has no stage buffer");
+    const int64_t kv_width = static_cast<int64_t>(layer->kv_heads) * D, q_width = static_cast<int64_t>(layer->q_heads) * D;
+    if (tokens > 1 && (k_stride < kv_width || v_stride < kv_width || (q != nullptr && (q_stride < q_width || q_out_stride < q_width))))
+        return fail(KVB_EINVAL, "kvb_rope_append: a row is longer than the distance to the next");
+    if (q != nullptr) {  // the queries are written while keys and values are read
+        const bool in_place = q == q_out && (tokens == 1 || q_stride == q_out_stride);
+        if (!in_place && rows_overlap(q, q_stride, q_width, q_out, q_out_stride, q_width, tokens))
+            return fail(KVB_EINVAL, "kvb_rope_append: q_out shares memory with q and is not q itself");
+        const Span written = rows_span(q_out, tokens, q_out_stride, q_width);
+        if (rows_overlap(k, k_stride, kv_width, q_out, q_out_stride, q_width, tokens) || rows_overlap(v, v_stride, kv_width, q_out, q_out_stride, q_width, tokens) ||
+            overlap(written, span_of(positions_dev, sizeof(int32_t) * static_cast<size_t>(tokens))) ||
+            overlap(written, span_of(rope->inv_freq, sizeof(double) * (rope->rotary_dim / 2))))
+            return fail(KVB_EINVAL, "kvb_rope_append: q_out shares memory with k, v, the positions or the frequencies");
+    }
+    AppendRope R{};
+    R.rope = {rope->inv_freq, rope->factor, rope->rotary_dim, rope->interleaved};
+    R.k_stride = k_stride;
+    R.v_stride = v_stride;
+    R.wide_k = rope_is_wide(*rope, D, k, k, k_stride, k_stride);
+    R.wide_v = v_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(v) & 15u) == 0;
+    if (q != nullptr) {
+        R.wide_q = rope_is_wide(*rope, D, q, q_out, q_stride, q_out_stride);
+        R.q = rope_rows_of(*rope, q, q_out, positions_dev, tokens, layer->q_heads, D, q_stride, q_out_stride, R.wide_q);
+    }
+    const LayerView V = make_view(*layer);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool bf = layer->dtype == KVB_DTYPE_BF16;
+    if (D == 128) return bf ? launch_rope_append<128, true>(V, R, k, v, positions_dev, tokens, s) : launch_rope_append<128, false>(V, R, k, v, positions_dev, tokens, s);
+    return bf ? launch_rope_append<256, true>(V, R, k, v, positions_dev, tokens, s) : launch_rope_append<256, false>(V, R, k, v, positions_dev, tokens, s);
 }
 
 extern "C" int kvb_decode_tile(const kvb_layer* layer, int tile, int head, void* out_k, void* out_v, void* stream) {

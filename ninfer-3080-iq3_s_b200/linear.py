@@ -1,0 +1,81 @@
+"""Linear attention with a decay for each head: the layers of a hybrid model that keep a state per sequence instead of a cache."""
+from __future__ import annotations
+
+import ctypes as C
+import functools
+
+import torch
+
+from . import capi
+from .cache import _ptr, _stream, row_stride
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(device, tokens, batch, v_heads, head_dim):
+    return capi.load().kvb_linear_workspace_bytes(tokens, batch, v_heads, head_dim)
+
+
+def _check_indices(n, **indices):
+    for name, x in indices.items():
+        if x.dtype != torch.int32 or x.shape != (n,) or not x.is_contiguous():
+            raise ValueError(f"{name}: int32 [{n}], got {tuple(x.shape)} of {x.dtype}")
+
+
+class LinearAttention:
+    """One layer: the decay of its heads and a pool of states, [slots, v_heads, head_dim of k, head_dim of v] in fp32, zeros at first."""
+
+    def __init__(self, qk_heads: int, v_heads: int, head_dim: int, log_decay: torch.Tensor, slots: int, dtype: torch.dtype = torch.bfloat16,
+                 device: str = "cuda"):
+        if tuple(log_decay.shape) != (v_heads,):
+            raise ValueError(f"log_decay: [{v_heads}], got {tuple(log_decay.shape)}")
+        self.qk_heads, self.v_heads, self.head_dim, self.slots, self.dtype = qk_heads, v_heads, head_dim, slots, dtype
+        self.device = torch.device(device)
+        self.state = torch.zeros((slots, v_heads, head_dim, head_dim), dtype=torch.float32, device=self.device)
+        self.log_decay = log_decay.to(device=self.device, dtype=torch.float32).contiguous()
+        self.error_word = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self.c = capi.kvb_linear(state=self.state.data_ptr(), log_decay=self.log_decay.data_ptr(), slots=slots, qk_heads=qk_heads, v_heads=v_heads,
+                                 head_dim=head_dim, dtype=capi.DTYPE_BF16 if dtype == torch.bfloat16 else capi.DTYPE_F16,
+                                 error_word=self.error_word.data_ptr())
+        self._ws = None
+
+    def _device_key(self) -> int:
+        return torch._C._cuda_getDevice() if self.device.type == "cuda" else -1
+
+    def _rows(self, q, k, v, out):
+        tokens = int(q.shape[0])
+        strides = [row_stride(x, h, self.head_dim, self.dtype, tokens) for x, h in ((q, self.qk_heads), (k, self.qk_heads), (v, self.v_heads))]
+        if out is None:
+            out = torch.empty((tokens, self.v_heads, self.head_dim), dtype=self.dtype, device=q.device)
+        elif out.shape != (tokens, self.v_heads, self.head_dim) or out.dtype != self.dtype or not out.is_contiguous():
+            raise ValueError(f"out: packed rows [{tokens}, {self.v_heads}, {self.head_dim}] of {self.dtype}")
+        return tokens, strides, out
+
+    def decode(self, q, k, v, scale: float, reads: torch.Tensor, writes: torch.Tensor, out=None) -> torch.Tensor:
+        """One token of each sequence: q, k [batch, qk_heads, head_dim], v [batch, v_heads, head_dim]; reads, writes: int32 [batch] on the device, the
+        slots a sequence's state is read from and written to (the same one for a step in place)."""
+        batch, (qs, ks, vs), out = self._rows(q, k, v, out)
+        _check_indices(batch, reads=reads, writes=writes)
+        capi.check(capi.load().kvb_linear_decode(C.byref(self.c), _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, batch, _ptr(reads), _ptr(writes), scale,
+                                                 _ptr(out), _stream()))
+        return out
+
+    def workspace(self, tokens: int, batch: int) -> torch.Tensor:
+        """Scratch for chunk calls.  One buffer per layer that only ever grows: a CUDA graph that captured its address stays valid as long as the
+        first call (made before the capture) asked for the largest shape the graph uses."""
+        n = _workspace_bytes(self._device_key(), tokens, batch, self.v_heads, self.head_dim)
+        if self._ws is None or self._ws.numel() * 4 < n:
+            self._ws = torch.empty((n + 3) // 4, dtype=torch.float32, device=self.device)
+        return self._ws
+
+    def chunk(self, q, k, v, offsets: torch.Tensor, scale: float, reads: torch.Tensor, writes: torch.Tensor, out=None) -> torch.Tensor:
+        """Several tokens of each sequence, packed: rows offsets[b] .. offsets[b + 1] - 1 are sequence b's; offsets: int32 [batch + 1] on the device."""
+        tokens, (qs, ks, vs), out = self._rows(q, k, v, out)
+        batch = int(reads.shape[0])
+        _check_indices(batch, reads=reads, writes=writes)
+        _check_indices(batch + 1, offsets=offsets)
+        capi.check(capi.load().kvb_linear_chunk(C.byref(self.c), _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(offsets), batch, tokens, _ptr(reads),
+                                                _ptr(writes), scale, _ptr(self.workspace(tokens, batch)), _ptr(out), _stream()))
+        return out
+
+    def errors(self) -> int:
+        return int(self.error_word.item())

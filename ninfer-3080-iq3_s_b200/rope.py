@@ -1,0 +1,39 @@
+"""Rotary positions: frequencies of the usual scalings for long contexts, and the turn of rows (kvb_rope_rows).  The append that turns keys on
+the way is KvarnLayer.rope_append."""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import capi
+from .cache import _ptr, _stream, check_positions, row_stride
+
+_SCALINGS = {"none": capi.ROPE_PLAIN, "linear": capi.ROPE_LINEAR, "ntk": capi.ROPE_NTK, "yarn": capi.ROPE_YARN}
+
+
+class Rope:
+    """The angles per position of a head's first `rotary_dim` dims, in device memory.  `scaling`: "none", "linear", "ntk" or "yarn", by `factor`
+    ("yarn" also wants `original`, the length the model was trained at)."""
+
+    def __init__(self, rotary_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, original: int = 0, interleaved: bool = False,
+                 device: str = "cuda"):
+        if scaling not in _SCALINGS:
+            raise ValueError(f"scaling {scaling!r}: one of {', '.join(_SCALINGS)}")
+        host, attention = (C.c_double * max(1, rotary_dim // 2))(), C.c_float()
+        capi.check(capi.load().kvb_rope_frequencies(rotary_dim, base, _SCALINGS[scaling], factor, original, host, C.byref(attention)))
+        self.rotary_dim, self.factor, self.interleaved = rotary_dim, attention.value, interleaved
+        self.inv_freq = torch.tensor(list(host), dtype=torch.float64).to(device)
+        self.c = capi.kvb_rope(inv_freq=self.inv_freq.data_ptr(), factor=self.factor, rotary_dim=rotary_dim, interleaved=int(interleaved))
+
+    def rows(self, x: torch.Tensor, positions: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+        """x: [tokens, heads, head_dim] (fp16 or bf16), packed or part of wider rows; positions: int32 [tokens] on the device.  `out` may be x."""
+        if x.dtype not in (torch.float16, torch.bfloat16) or x.dim() != 3:
+            raise ValueError(f"x: rows [tokens, heads, head_dim] of float16 or bfloat16, got {tuple(x.shape)} of {x.dtype}")
+        tokens, heads, dim = x.shape
+        check_positions(positions, tokens)
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+        capi.check(capi.load().kvb_rope_rows(C.byref(self.c), _ptr(x), row_stride(x, heads, dim, x.dtype), _ptr(out),
+                                             row_stride(out, heads, dim, x.dtype, tokens), _ptr(positions), tokens, heads, dim,
+                                             capi.DTYPE_BF16 if x.dtype == torch.bfloat16 else capi.DTYPE_F16, _stream()))
+        return out
