@@ -135,7 +135,11 @@ int linear_call(const kvb_linear* layer, const char* who, const void* q, int64_t
     V.head_dim = D;
     V.error_word = layer->error_word;
     const bool bf = layer->dtype == KVB_DTYPE_BF16;
-    (void)workspace;
+    if (static_cast<int64_t>(tokens) > 16 * static_cast<int64_t>(batch)) {
+        if (workspace == nullptr) return fail(KVB_EINVAL, "%s: null workspace", who);
+        const bool aligned = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) == 0 && q_stride % 8 == 0 && k_stride % 8 == 0 && v_stride % 8 == 0;
+        return linear_chunks(V, bf, aligned, workspace, stream);
+    }
     if (D == 128) return static_cast<int64_t>(batch) * layer->v_heads < 2 * device_sm_count() ? launch_step<128, 32>(V, bf, stream) : launch_step<128, 128>(V, bf, stream);
     return static_cast<int64_t>(batch) * layer->v_heads < 2 * device_sm_count() ? launch_step<64, 16>(V, bf, stream) : launch_step<64, 64>(V, bf, stream);
 }
@@ -159,6 +163,9 @@ extern "C" int kvb_linear_chunk(const kvb_linear* layer, const void* q, int64_t 
 }
 
 extern "C" size_t kvb_linear_workspace_bytes(int tokens, int batch, int v_heads, int head_dim) {
-    (void)tokens, (void)batch, (void)v_heads, (void)head_dim;
-    return kvb::kWorkspaceSlack;
+    using namespace kvb;
+    if (tokens < 1 || batch < 1 || v_heads < 1 || (head_dim != 64 && head_dim != 128)) return kWorkspaceSlack;
+    const int segment = linear_segment(tokens, batch, v_heads);
+    if (tokens <= segment) return kWorkspaceSlack;
+    return sizeof(float) * static_cast<size_t>(linear_units(tokens, batch, segment)) * v_heads * head_dim * head_dim + kWorkspaceSlack;
 }

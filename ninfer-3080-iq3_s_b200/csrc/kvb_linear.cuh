@@ -8,6 +8,7 @@
 namespace kvb {
 
 constexpr int kMostSequences = 256;  // of one call
+constexpr int kLinearChunk = 128;    // tokens that the chunked form takes at a time
 
 // Rows [begin, end) of one sequence and the slots its state is read from and written to.
 struct Sequence {
@@ -58,6 +59,11 @@ struct LinearView {
         return false;
     }
 };
+
+// The chunked form: tokens of a segment (a multiple of a chunk), the grid's units (segments of all sequences, at most), and the launches.
+int linear_segment(int tokens, int batch, int v_heads);
+int linear_units(int tokens, int batch, int segment);
+int linear_chunks(const LinearView& V, bool bf16, bool aligned, void* workspace, cudaStream_t stream);
 
 int check_linear(const kvb_linear* layer, const char* who);
 
