@@ -8,7 +8,7 @@
 namespace kvb {
 
 constexpr int kMostSequences = 256;  // of one call
-constexpr int kLinearChunk = 128;    // tokens that the chunked form takes at a time
+constexpr int kLinearChunk = 64;     // tokens that the chunked form takes at a time
 
 // Rows [begin, end) of one sequence and the slots its state is read from and written to.
 struct Sequence {

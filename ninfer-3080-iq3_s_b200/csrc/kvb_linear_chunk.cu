@@ -1,21 +1,35 @@
 // kvb_linear_chunk.cu -- linear attention with a decay for each head over prompts, chunk by chunk on the 5th-generation tensor cores.
 //
-// For a chunk of C = 128 tokens (rows i, j; L of them valid) behind a state S, with lambda = exp(log_decay):
+// For a chunk of C = 64 tokens (rows i, j; L of them valid) behind a state S, with lambda = exp(log_decay):
 //
 //   P_ij  = lambda^(i-j) q_i k_j  (j <= i, else 0)                        scores          C x C
 //   o_i   = scale (sum_j P_ij v_j + lambda^(i+1) q_i S)                   inside + before
 //   S    <- lambda^L S + sum_j (lambda^(L-1-j) k_j) v_j^T                 the state behind the chunk
 //
 // Everything but the scores is computed transposed, head dims of v along the M rows of the MMAs: S^T stays in tensor memory as an fp32 accumulator from
-// chunk to chunk, and is an A operand there too (two 16-bit numbers an element, whose sum has 16 bits of bf16 or 22 of fp16); only rows of
-// tokens as they come from global memory, decayed keys (two 16-bit numbers likewise, so that states keep their precision over long prompts) and P lie in
-// shared memory.  P is rounded to the type once, like the output.  Heads of 64 dims fill both halves of the M rows with the same 64.
+// chunk to chunk, and is an A operand there too; only rows of tokens as they come from global memory, decayed keys and P lie in shared memory.
+// Roundings: P, and the state as an operand, to the type, like the output that they are summed up to (both together as much as the output's own
+// rounding); decayed keys as two numbers of the type, whose sum has 16 bits of bf16 or 22 of fp16, so that states keep their precision over long prompts.  Heads of 64 dims fill both halves of the M rows with the same 64; the
+// scores' 64 rows are the first of 128, and what the others multiply is not looked at.
+//
+// Warps by role, so that a chunk's steps run beside its neighbours':
+//   state warps   the state as an operand (then decayed over the chunk), decayed keys of the next chunk
+//   score warps   P, a chunk ahead
+//   row warps     outputs
+//   an MMA warp   P V and the next chunk's scores while the state becomes an operand; then S += K'^T V and the outputs' part from before
+//   a load warp   tiles by TMA, into three stages (16-byte copies by the lanes filled the SM's load queue, where everybody's shared-memory accesses
+//                 and arrivals waited behind them: 5,400 cycles a chunk)
+//   store warps   outputs, 16 bytes a lane (two bytes a lane from the row warps held those up for 4,000 cycles a chunk, most of it in the fence before
+//                 the next P, which waits for the thread's stores)
+// The loop that cannot be shortened is state -> operand -> two products -> state.
 //
 // A sequence is split into segments where there are fewer heads and sequences than SMs: a first launch sums up each segment alone
 // (keys and values only, half the reads of the second), the second starts each from the sums before it.
 //
 // In fp16 the scores of a row and the state's rows are scaled by a power of two to a largest magnitude of 2^14 .. 2^15 before they are rounded, so that
 // neither overflows; the scales come out again in the sum of the two parts.  bf16 has the range of fp32.
+#include <cuda.h>
+
 #include "kvb_linear.cuh"
 #include "kvb_tcgen05.cuh"
 
@@ -23,32 +37,41 @@ namespace kvb {
 namespace {
 
 constexpr int kC = kLinearChunk;  // tokens of a chunk
-constexpr int kComputeWarps = 8, kMmaWarp = 8, kLoadWarps = 4;
-constexpr int kComputeThreads = kComputeWarps * 32, kLoadThreads = kLoadWarps * 32;
-constexpr int kChunkThreads = kComputeThreads + 32 + kLoadThreads;
+constexpr int kStages = 3;
+constexpr int kStateWarps = 8, kRowWarps = 8;
+// the last eight: warp 0, 1, 4, 5 of them P (rows 0 .. 63 of tensor memory are a warp's by its number mod 4), 2 MMAs, 3 loads, 6, 7 stores of even and odd chunks
+constexpr int kLastWarps = kStateWarps + kRowWarps, kMmaWarp = kLastWarps + 2, kLoadWarp = kLastWarps + 3, kStoreWarp = kLastWarps + 6;
+constexpr int kStateThreads = kStateWarps * 32, kRowThreads = kRowWarps * 32, kScoreThreads = 128;
+constexpr int kChunkThreads = (kLastWarps + 8) * 32;  // 24 warps: six to a scheduler, 80 registers a thread
 constexpr uint32_t kTmemCols = 512;
 
 template <int D> struct LinearSmem {
-    static constexpr int kTileBytes = kC * D * 2;  // [D / 64][128 rows][128 bytes], 128-byte swizzle
-    alignas(1024) unsigned char q[2][kTileBytes];
-    unsigned char k[2][kTileBytes];                // keys, then the first numbers of the decayed keys
-    unsigned char v[2][kTileBytes];
-    unsigned char x[kC * kC * 2];                  // the second numbers of the decayed keys, then P
-    float power[kC];                               // lambda^n
-    float before[kC];                              // scale lambda^(i + 1)
-    float inside[kC];                              // scale times what P's row i was scaled down by (fp16)
-    uint16_t most[2][2][kC];                       // exponents of the largest magnitudes of a row of the state, of P, one a column half (fp16)
-    uint64_t full[2], empty[2], keys_ready[2], scores, state_ready, scores_read, state_done, p_ready, out_full, out_read, most_ready[2], drained;
+    static constexpr int kTileBytes = kC * D * 2;  // [D / 64][64 rows][128 bytes], 128-byte swizzle
+    struct Stage {  // the scores' MMA reads 64 rows behind those of q, too
+        unsigned char q[kTileBytes], k[kTileBytes], v[kTileBytes];
+    };
+    alignas(1024) Stage stage[kStages];    // the keys' place takes the first numbers of the decayed keys once the scores are there
+    unsigned char second[2][kTileBytes];   // their second numbers, of two chunks
+    unsigned char p[2][kC * kC * 2];       // P of two chunks
+    uint32_t out[2][kTileBytes / 4];       // outputs of two chunks, [32 pairs of tokens][D]
+    float fade[2][2 * kC];                 // fade[s][x] = lambda^(63 - x - s), 0 behind lambda^0; the second copy for aligned pairs from odd x on
+    float before[kC];                      // scale lambda^(i + 1)
+    float inside[2][kC];                   // scale times what P's row i was scaled down by (fp16)
+    uint8_t up[3][128];                    // exponent field of what a row of the state was scaled down by (fp16)
+    uint8_t most_state[2][128], most_p[2][2][kC];  // exponents of the largest magnitudes of a row, one a column half (fp16)
+    // chunk c has the one of c mod their number; `done`: all products of a chunk
+    uint64_t full[kStages], done[kStages], state_ready[3], scores[2], p_ready[2], keys_ready[2], out_read[2], out_ready[2], out_free[2], most_ready[2], drained;
     uint32_t tmem_base;
     int abort_flag;
     int unit[3];
 };
 
 struct ChunkCall {
+    CUtensorMap q, k, v;  // [tokens][heads * D], boxes of 64 rows of 64 dims
     LinearView V;
     float* sums;   // [unit][head][D][D]: each segment's sum; the last one's place holds the state before the first
     int segment;   // tokens, a multiple of kC
-    bool aligned;  // rows of q, k, v keep to 16 bytes
+    bool aligned;  // rows of q, k, v keep to 16 bytes: the maps are there
 };
 
 // Sequence and segment of the call's unit `unit`, found by one warp; the same for all threads afterwards.  seq = batch: none.
@@ -101,45 +124,48 @@ template <bool kBf16> __device__ __forceinline__ float2 unpack_pair(uint32_t w) 
     if constexpr (kBf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
     else return unpack_half2(w);
 }
+template <bool kBf16> __device__ __forceinline__ F2 pair_of(uint32_t w) {
+    const float2 f = unpack_pair<kBf16>(w);
+    return F2(f.x, f.y);
+}
+template <bool kBf16> __device__ __forceinline__ uint32_t pack_pair(F2 x) {
+    const float2 f = x.get();
+    return pack_pair<kBf16>(f.x, f.y);
+}
+__device__ __forceinline__ F2 pair_of_words(uint32_t a, uint32_t b) { return F2(__uint_as_float(a), __uint_as_float(b)); }
 // Instruction descriptor of 16-bit operands of either type (format 0 = f16, 1 = bf16).
 template <bool kBf16> __host__ __device__ constexpr uint32_t idesc_16(int m, int n, bool a_mn, bool b_mn) {
     return tc::idesc_f16(m, n, a_mn, b_mn) | (kBf16 ? (1u << 7) | (1u << 10) : 0u);
 }
-// 2^-e and 2^e for the e that brings magnitudes with this largest exponent field below 2^15; 1 where it is 0's or not finite.
-__device__ __forceinline__ float2 down_and_up(int field) {
+// Exponent fields of 2^-e and 2^e for the e that brings magnitudes with this largest exponent field below 2^15; 1 where it is 0's or not finite.
+__device__ __forceinline__ float of_field(int field) { return __uint_as_float(static_cast<uint32_t>(field) << 23); }
+__device__ __forceinline__ int2 down_and_up(int field) {
     const int e = field > 0 && field < 255 ? max(-112, min(112, field - 127 - 14)) : 0;
-    return make_float2(__uint_as_float(static_cast<uint32_t>(127 - e) << 23), __uint_as_float(static_cast<uint32_t>(127 + e) << 23));
+    return make_int2(127 - e, 127 + e);
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// A box of a tensor map into shared memory, from `row` and the first dim `x` on (a multiple of 64).
+__device__ __forceinline__ void tma_load(unsigned char* dst, const CUtensorMap& map, int x, int row, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+                 "l"(reinterpret_cast<uint64_t>(&map)), "r"(x), "r"(row), "r"(smem_u32(bar))
+                 : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kLeft> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
-
-// Rows of a chunk into a tile, zeros behind the valid ones.
-template <int D> __device__ __forceinline__ void load_tile(unsigned char* tile, const uint16_t* rows, int64_t stride, int valid, bool aligned) {
-    constexpr int kUnits = D / 8;  // 16 bytes each, of a row
-    const int tid = threadIdx.x - kComputeThreads - 32;
-    if (aligned) {
-        const uint32_t base = smem_u32(tile);
-#pragma unroll 8
-        for (int u = tid; u < kC * kUnits; u += kLoadThreads) {
-            const int row = u / kUnits, c = u % kUnits;
-            const bool in = row < valid;
-            cp_async16(base + (c >> 3) * (kC * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4), rows + (in ? row : 0) * stride + 8 * c, in ? 16u : 0u);
-        }
-    } else {
-        for (int u = tid; u < kC * kUnits; u += kLoadThreads) {
-            const int row = u / kUnits, c = u % kUnits;
-            uint32_t w[4] = {0u, 0u, 0u, 0u};
-            if (row < valid) {
-                const uint16_t* from = rows + row * stride + 8 * c;
+template <int D> __device__ __forceinline__ void load_tile(unsigned char* tile, const CUtensorMap& map, int head, int64_t token, uint64_t* bar) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = static_cast<uint32_t>(from[2 * e]) | static_cast<uint32_t>(from[2 * e + 1]) << 16;
-            }
-            *reinterpret_cast<uint4*>(tile + (c >> 3) * (kC * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int half = 0; half < D / 64; ++half) tma_load(tile + half * kC * 128, map, head * D + 64 * half, static_cast<int>(token), bar);
+}
+// The same by a warp for rows that do not keep to 16 bytes.
+template <int D> __device__ __noinline__ void load_tile_by_elements(unsigned char* tile, const uint16_t* rows, int64_t stride, int valid, int lane) {
+    constexpr int kUnits = D / 8;
+    for (int u = lane; u < kC * kUnits; u += 32) {
+        const int row = u / kUnits, c = u % kUnits;
+        uint32_t w[4] = {0u, 0u, 0u, 0u};
+        if (row < valid) {
+            const uint16_t* from = rows + row * stride + 8 * c;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = static_cast<uint32_t>(from[2 * e]) | static_cast<uint32_t>(from[2 * e + 1]) << 16;
         }
+        *reinterpret_cast<uint4*>(tile + (c >> 3) * (kC * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
@@ -147,7 +173,7 @@ template <int D> __device__ __forceinline__ void load_tile(unsigned char* tile, 
 template <bool kBf16> __device__ __noinline__ float inside_again(const unsigned char* p, int i, const uint16_t* v, int64_t stride) {
     float sum = 0.0f;
     for (int j = 0; j <= i; ++j) {
-        const uint16_t w = *reinterpret_cast<const uint16_t*>(p + (j >> 6) * (kC * 128) + i * 128 + ((((j & 63) >> 3) ^ (i & 7)) << 4) + (j & 7) * 2);
+        const uint16_t w = *reinterpret_cast<const uint16_t*>(p + i * 128 + (((j >> 3) ^ (i & 7)) << 4) + (j & 7) * 2);
         sum = fmaf(in_to_f32<kBf16>(w), in_to_f32<kBf16>(v[j * stride]), sum);
     }
     return sum;
@@ -155,11 +181,11 @@ template <bool kBf16> __device__ __noinline__ float inside_again(const unsigned 
 
 // kSums: the first launch, sums of segments; else the outputs and the state behind each sequence.
 template <int D, bool kBf16, bool kSums>
-__global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const ChunkCall P) {
+__global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_constant__ ChunkCall P) {
     using Smem = LinearSmem<D>;
-    constexpr int kHalf = D / 2;                    // columns of the state a compute warp has
-    constexpr uint32_t kStateCol = 0, kFirstCol = D, kSecondCol = D + D / 2, kScoreCol = 2 * D, kOutCol = 2 * D + kC;
-    static_assert(kOutCol + kC <= kTmemCols, "tensor memory");
+    constexpr int kHalf = D / 2;  // columns of the state a state warp has
+    constexpr uint32_t kStateCol = 0, kOperandCol = D, kScoreCol = D + D / 2, kBeforeCol = kScoreCol + kC, kInsideCol = kBeforeCol + 2 * kC;
+    static_assert(kInsideCol + 2 * kC <= kTmemCols, "tensor memory");
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
     grid_dependency_wait();
@@ -185,115 +211,156 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const ChunkCall
 
     if (warp == kMmaWarp) tc::tmem_alloc(&sm.tmem_base, kTmemCols);
     if (threadIdx.x == 0) {
-        for (int s = 0; s < 2; ++s) {
-            mbar_init(&sm.full[s], kLoadThreads);
-            mbar_init(&sm.empty[s], 1);
-            mbar_init(&sm.keys_ready[s], kComputeThreads);
-            mbar_init(&sm.most_ready[s], kComputeThreads);
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&sm.full[s], 1);
+            mbar_init(&sm.done[s], 1);
+            mbar_init(&sm.state_ready[s], kStateThreads);
         }
-        mbar_init(&sm.scores, 1);
-        mbar_init(&sm.state_done, 1);
-        mbar_init(&sm.out_full, 1);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&sm.scores[s], 1);
+            mbar_init(&sm.p_ready[s], kScoreThreads);
+            mbar_init(&sm.keys_ready[s], kStateThreads);
+            mbar_init(&sm.out_read[s], kRowThreads);
+            mbar_init(&sm.out_ready[s], kRowThreads);
+            mbar_init(&sm.out_free[s], 1);
+        }
+        mbar_init(&sm.most_ready[0], kStateThreads);
+        mbar_init(&sm.most_ready[1], kScoreThreads);
         mbar_init(&sm.drained, 1);
-        mbar_init(&sm.state_ready, kComputeThreads);
-        mbar_init(&sm.scores_read, kComputeThreads);
-        mbar_init(&sm.p_ready, kComputeThreads);
-        mbar_init(&sm.out_read, kComputeThreads);
         mbar_fence_init();
         sm.abort_flag = 0;
     }
-    if (threadIdx.x < kC) {
-        const int n = threadIdx.x;
-        sm.power[n] = decay_power(g, n);
-        sm.before[n] = V.scale * decay_power(g, n + 1);
-        sm.inside[n] = V.scale;
+    if (threadIdx.x < 4 * kC) {
+        const int copy = threadIdx.x / (2 * kC), x = threadIdx.x % (2 * kC), n = kC - 1 - x - copy;
+        sm.fade[copy][x] = n >= 0 ? decay_power(g, n) : 0.0f;
+        if (threadIdx.x < kC) sm.before[threadIdx.x] = V.scale * decay_power(g, threadIdx.x + 1);
     }
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = sm.tmem_base;
     bool failed = false;
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (!failed && !chunk_wait(bar, parity, &sm.abort_flag)) failed = true;
+    auto wait = [&](uint64_t* bar, int phase) {
+        if (!failed && !chunk_wait(bar, static_cast<uint32_t>(phase & 1), &sm.abort_flag)) failed = true;
         return !failed;
     };
+    auto wait2 = [&](uint64_t (&bars)[2], int c) { return wait(&bars[c & 1], c >> 1); };
+    auto wait3 = [&](uint64_t (&bars)[3], int c) { return wait(&bars[c % 3], c / 3); };
 
-    if (warp > kMmaWarp) {
-        // ---- loads: chunk c into stage c & 1; a chunk is announced once its copies have landed, a chunk later
-        const uint16_t* const q = V.q + static_cast<int64_t>(head / V.share) * D;
-        const uint16_t* const k = V.k + static_cast<int64_t>(head / V.share) * D;
-        const uint16_t* const v = V.v + static_cast<int64_t>(head) * D;
+    if (warp == kLoadWarp) {
+        // ---- loads: chunk c into stage c % 3.  Rows behind a sequence's last come with it, whatever they hold: see there.
+        const int qk_head = head / V.share;
         for (int c = 0; c < chunks; ++c) {
-            const int st = c & 1, t = begin + c * kC, valid = min(kC, end - t);
-            if (c > 1 && !wait(&sm.empty[st], ((c >> 1) + 1) & 1)) break;
-            load_tile<D>(sm.k[st], k + t * V.k_stride, V.k_stride, valid, P.aligned);
-            load_tile<D>(sm.v[st], v + t * V.v_stride, V.v_stride, valid, P.aligned);
-            if (!kSums) load_tile<D>(sm.q[st], q + t * V.q_stride, V.q_stride, valid, P.aligned);
-            cp_async_commit();
-            if (c > 0) {
-                cp_async_wait<1>();
+            const int stage = c % kStages;
+            typename Smem::Stage& st = sm.stage[stage];
+            const int64_t t = begin + c * kC;
+            if (c >= kStages && !wait3(sm.done, c - kStages)) break;
+            if (P.aligned) {
+                if (lane == 0) {
+                    mbar_expect_tx(&sm.full[stage], (kSums ? 2 : 3) * Smem::kTileBytes);
+                    load_tile<D>(st.k, P.k, qk_head, t, &sm.full[stage]);
+                    if (!kSums) load_tile<D>(st.q, P.q, qk_head, t, &sm.full[stage]);
+                    load_tile<D>(st.v, P.v, head, t, &sm.full[stage]);
+                }
+            } else {
+                const int valid = min(kC, end - static_cast<int>(t));
+                load_tile_by_elements<D>(st.k, V.k + t * V.k_stride + qk_head * D, V.k_stride, valid, lane);
+                if (!kSums) load_tile_by_elements<D>(st.q, V.q + t * V.q_stride + qk_head * D, V.q_stride, valid, lane);
+                load_tile_by_elements<D>(st.v, V.v + t * V.v_stride + head * D, V.v_stride, valid, lane);
                 fence_proxy_async();
-                mbar_arrive(&sm.full[st ^ 1]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.full[stage]);
             }
+            __syncwarp();
         }
-        cp_async_wait<0>();
-        fence_proxy_async();
-        if (!failed && chunks > 0) mbar_arrive(&sm.full[(chunks - 1) & 1]);
+        // no copy lands in shared memory that is no longer this CTA's
+        if (failed && P.aligned)
+            for (int c = max(0, chunks - kStages); c < chunks; ++c) mbar_wait_bounded(&sm.full[c % kStages], (c / kStages) & 1);
+    } else if (warp == kStoreWarp || warp == kStoreWarp + 1) {
+        // ---- stores: outputs of even chunks, of odd ones
+        const bool wide = (reinterpret_cast<uintptr_t>(V.out) & 15u) == 0;
+        const int64_t out_stride = static_cast<int64_t>(V.v_heads) * D;
+        for (int c = warp - kStoreWarp; !kSums && c < chunks; c += 2) {
+            const int64_t t = begin + c * kC;
+            const int valid = min(kC, end - static_cast<int>(t));
+            if (!wait2(sm.out_ready, c)) break;
+            uint16_t* const to = V.out + (t * V.v_heads + head) * D;
+            const uint32_t* const words = sm.out[c & 1];  // of a head dim and two tokens
+            if (wide) {
+                constexpr int kUnits = D / 8, kAtOnce = 4;  // 8 dims a unit
+#pragma unroll 1
+                for (int u0 = lane; u0 < kC / 2 * kUnits; u0 += 32 * kAtOnce) {
+                    uint4 r[kAtOnce][2];
+#pragma unroll
+                    for (int n = 0; n < kAtOnce; ++n) {
+                        r[n][0] = reinterpret_cast<const uint4*>(words)[2 * (u0 + 32 * n)];
+                        r[n][1] = reinterpret_cast<const uint4*>(words)[2 * (u0 + 32 * n) + 1];
+                    }
+#pragma unroll
+                    for (int n = 0; n < kAtOnce; ++n) {
+                        const int row = (u0 + 32 * n) / kUnits * 2, col = (u0 + 32 * n) % kUnits;
+                        uint16_t* const at = to + row * out_stride + 8 * col;
+                        const uint4 x = r[n][0], y = r[n][1];
+                        if (row < valid) *reinterpret_cast<uint4*>(at) = make_uint4(prmt(x.x, x.y, 0x5410), prmt(x.z, x.w, 0x5410), prmt(y.x, y.y, 0x5410), prmt(y.z, y.w, 0x5410));
+                        if (row + 1 < valid)
+                            *reinterpret_cast<uint4*>(at + out_stride) = make_uint4(prmt(x.x, x.y, 0x7632), prmt(x.z, x.w, 0x7632), prmt(y.x, y.y, 0x7632), prmt(y.z, y.w, 0x7632));
+                    }
+                }
+            } else {
+#pragma unroll 1
+                for (int u = lane; u < valid * D; u += 32) to[u / D * out_stride + u % D] = static_cast<uint16_t>(words[u / D / 2 * D + u % D] >> (u / D % 2 * 16));
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.out_free[c & 1]);
+        }
     } else if (warp == kMmaWarp) {
         // ---- MMAs, issued by one thread
-        const uint64_t q0 = tc::smem_desc(smem_u32(sm.q[0]), 16, 1024), k0 = tc::smem_desc(smem_u32(sm.k[0]), 16, 1024), p0 = tc::smem_desc(smem_u32(sm.x), 16, 1024);
-        // MN-major: the next 64 head dims a tile half further (heads of 64 dims: the same ones again), the next 8 tokens 1024 bytes
-        const uint64_t v0 = tc::smem_desc(smem_u32(sm.v[0]), D == 128 ? kC * 128 : 0, 1024);
-        const uint64_t key0 = tc::smem_desc(smem_u32(sm.k[0]), kC * 128, 1024);
-        const uint64_t second0 = kSums ? tc::smem_desc(smem_u32(sm.q[0]), kC * 128, 1024) : tc::smem_desc(smem_u32(sm.x), kC * 128, 1024);
+        // MN-major: the next 64 head dims half a tile further (heads of 64 dims: the same ones again), the next 8 tokens 1024 bytes
         constexpr uint32_t kScores = idesc_16<kBf16>(128, kC, false, false), kState = idesc_16<kBf16>(128, D, true, true), kOut = idesc_16<kBf16>(128, kC, true, false);
+        auto rows_desc = [&](const unsigned char* tile) { return tc::smem_desc(smem_u32(tile), 16, 1024); };
+        auto dims_desc = [&](const unsigned char* tile) { return tc::smem_desc(smem_u32(tile), D == 128 ? kC * 128 : 0, 1024); };
         auto k_major = [](uint64_t desc, int step) { return tc::desc_at(desc, (step >> 2) * (kC * 128) + (step & 3) * 32); };  // 16 of the K dims further
-        for (int c = 0; c < chunks; ++c) {
-            const int st = c & 1, at = st * Smem::kTileBytes;
-            if (!kSums) {
-                if (!wait(&sm.full[st], (c >> 1) & 1)) break;
-                if (c > 0 && !wait(&sm.out_read, (c - 1) & 1)) break;
-                tc::fence_after_sync();
-                if (tc::elect_one()) {
-                    const uint64_t a = tc::desc_here(tc::desc_at(q0, at)), b = tc::desc_here(tc::desc_at(k0, at));
-#pragma unroll
-                    for (int s = 0; s < D / 16; ++s) tc::mma_f16_ss(tmem + kScoreCol, k_major(a, s), k_major(b, s), kScores, s > 0);
-                    tc::commit(&sm.scores);
-                }
-                __syncwarp();
-                if (!wait(&sm.state_ready, c & 1)) break;
-            }
-            if (!wait(&sm.keys_ready[st], (c >> 1) & 1)) break;
+        auto issue_scores = [&](int c) {
+            const typename Smem::Stage& st = sm.stage[c % kStages];
+            if (!wait3(sm.full, c)) return;
             tc::fence_after_sync();
             if (tc::elect_one()) {
-                const uint64_t a = tc::desc_here(tc::desc_at(v0, at)), b = tc::desc_here(tc::desc_at(key0, at)), b2 = tc::desc_here(kSums ? tc::desc_at(second0, at) : second0);
+                const uint64_t a = tc::desc_here(rows_desc(st.q)), b = tc::desc_here(rows_desc(st.k));
+#pragma unroll
+                for (int s = 0; s < D / 16; ++s) tc::mma_f16_ss(tmem + kScoreCol, k_major(a, s), k_major(b, s), kScores, s > 0);
+                tc::commit(&sm.scores[c & 1]);
+            }
+            __syncwarp();
+        };
+        if (!kSums && chunks > 0) issue_scores(0);
+        for (int c = 0; c < chunks && !failed; ++c) {
+            const typename Smem::Stage& st = sm.stage[c % kStages];
+            if (!wait2(sm.keys_ready, c)) break;
+            if (!kSums) {  // beside the state's way into an operand: what does not need it
+                if (!wait2(sm.p_ready, c) || (c > 1 && !wait2(sm.out_read, c - 2))) break;
+                tc::fence_after_sync();
+                if (tc::elect_one()) {
+                    const uint64_t a = tc::desc_here(dims_desc(st.v)), b = tc::desc_here(rows_desc(sm.p[c & 1]));
+#pragma unroll
+                    for (int s = 0; s < kC / 16; ++s) tc::mma_f16_ss(tmem + kInsideCol + (c & 1) * kC, tc::desc_at(a, s * 2048), k_major(b, s), kOut, s > 0);
+                }
+                __syncwarp();
+                if (c + 1 < chunks) issue_scores(c + 1);
+                if (!wait3(sm.state_ready, c)) break;
+            }
+            tc::fence_after_sync();
+            if (tc::elect_one()) {
+                const uint64_t a = tc::desc_here(dims_desc(st.v)), b = tc::desc_here(tc::smem_desc(smem_u32(st.k), kC * 128, 1024)), b2 = tc::desc_here(tc::smem_desc(smem_u32(sm.second[c & 1]), kC * 128, 1024));
 #pragma unroll
                 for (int s = 0; s < kC / 16; ++s) tc::mma_f16_ss(tmem + kStateCol, tc::desc_at(a, s * 2048), tc::desc_at(b, s * 2048), kState, !kSums || c > 0 || s > 0);
 #pragma unroll
                 for (int s = 0; s < kC / 16; ++s) tc::mma_f16_ss(tmem + kStateCol, tc::desc_at(a, s * 2048), tc::desc_at(b2, s * 2048), kState, true);
-                if (kSums) tc::commit(&sm.empty[st]);
-                if (!kSums || c == chunks - 1) tc::commit(&sm.state_done);
-            }
-            __syncwarp();
-            if (kSums) continue;
-            if (!wait(&sm.scores_read, c & 1)) break;
-            tc::fence_after_sync();
-            if (tc::elect_one()) {
-                const uint64_t b = tc::desc_here(tc::desc_at(q0, at));
+                if (!kSums) {
+                    const uint64_t q = tc::desc_here(rows_desc(st.q));
 #pragma unroll
-                for (int s = 0; s < D / 16; ++s) tc::mma_f16_ts(tmem + kScoreCol, tmem + kFirstCol + 8 * s, k_major(b, s), kScores, s > 0);
-#pragma unroll
-                for (int s = 0; s < D / 16; ++s) tc::mma_f16_ts(tmem + kScoreCol, tmem + kSecondCol + 8 * s, k_major(b, s), kScores, true);
-            }
-            __syncwarp();
-            if (!wait(&sm.p_ready, c & 1)) break;
-            tc::fence_after_sync();
-            if (tc::elect_one()) {
-                const uint64_t a = tc::desc_here(tc::desc_at(v0, at)), b = tc::desc_here(p0);
-#pragma unroll
-                for (int s = 0; s < kC / 16; ++s) tc::mma_f16_ss(tmem + kOutCol, tc::desc_at(a, s * 2048), k_major(b, s), kOut, s > 0);
-                tc::commit(&sm.out_full);
-                tc::commit(&sm.empty[st]);
+                    for (int s = 0; s < D / 16; ++s) tc::mma_f16_ts(tmem + kBeforeCol + (c & 1) * kC, tmem + kOperandCol + 8 * s, k_major(q, s), kScores, s > 0);
+                }
+                tc::commit(&sm.done[c % 3]);
             }
             __syncwarp();
         }
@@ -302,14 +369,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const ChunkCall
             __syncwarp();
             mbar_wait_bounded(&sm.drained, 0);
         }
-    } else {
-        // ---- the eight other warps: rows 32 (warp % 4) + lane of tensor memory, columns by warp / 4
+    } else if (warp < kStateWarps) {
+        // ---- state warps: rows 32 (warp % 4) + lane of S^T, columns by warp / 4
         const int quad = warp & 3, side = warp >> 2, row = 32 * quad + lane, dim = row % D, tid = threadIdx.x;
         const uint32_t lanes = static_cast<uint32_t>(32 * quad) << 16;
         const uint32_t state_at = tmem + lanes + kStateCol + side * kHalf;
 
         if (!kSums || last_segment) {
-            // the state before the segment, rows of S^T: from the pool, or the sums of the segments before
+            // the state before the segment: from the pool, or the sums of the segments before
             const float* from = V.state_of(seq.from, head);
             if (!kSums && unit.count > 1 && unit.index == 0) from = sums + (unit.count - 1) * sums_step;
 #pragma unroll 1
@@ -323,6 +390,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const ChunkCall
                     float f[32];
 #pragma unroll
                     for (int e = 0; e < 32; ++e) f[e] = 0.0f;
+#pragma unroll 1
                     for (int s = 0; s < unit.index; ++s) {
                         const float* sum = sums - (unit.index - s) * sums_step;
                         const float w = decay_power(g, (unit.index - 1 - s) * P.segment);
@@ -343,14 +411,50 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const ChunkCall
             }
             tc::tmem_st_wait();
         }
-        for (int c = 0; c < chunks; ++c) {
-            const int st = c & 1, t = begin + c * kC, valid = min(kC, end - t);
-            float up = 1.0f;  // what this row of the state was scaled down by
-            if (!kSums) {
-                // ---- the state as an operand, and decayed over the chunk
-                if (c > 0 && !wait(&sm.state_done, (c - 1) & 1)) break;
+        // decayed keys of chunk c, two numbers each
+        auto decay_keys = [&](int c) {
+            if (!wait3(sm.full, c)) return;
+            if (!kSums && !wait2(sm.scores, c)) return;  // the keys themselves have been read
+            const int t = begin + c * kC, valid = min(kC, end - t);
+            unsigned char* const keys = sm.stage[c % kStages].k;
+            unsigned char* const second = sm.second[c & 1];
+            constexpr int kEach = kC * D / 8 / kStateThreads;
+#pragma unroll
+            for (int n = 0; n < kEach; ++n) {
+                const int u = tid + n * kStateThreads, j = (u >> 3) & (kC - 1);
+                const float w = kSums ? decay_power(g, end - 1 - t - j) : sm.fade[0][kC - 1 - max(valid - 1 - j, 0)];
+                uint4 raw = *reinterpret_cast<const uint4*>(keys + 16 * u);
+                if (j >= valid) raw = make_uint4(0u, 0u, 0u, 0u);
+                const uint32_t in[4] = {raw.x, raw.y, raw.z, raw.w};
+                uint32_t a[4], b[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const F2 x = mul2(pair_of<kBf16>(in[e]), F2(w, w));
+                    a[e] = pack_pair<kBf16>(x);
+                    b[e] = pack_pair<kBf16>(sub2(x, pair_of<kBf16>(a[e])));
+                }
+                *reinterpret_cast<uint4*>(keys + 16 * u) = make_uint4(a[0], a[1], a[2], a[3]);
+                *reinterpret_cast<uint4*>(second + 16 * u) = make_uint4(b[0], b[1], b[2], b[3]);
+            }
+            if (valid < kC) {  // values behind the sequence's last row meet zeros in P and the keys: they have to be finite
+                for (int u = tid; u < kC * D / 8; u += kStateThreads)
+                    if (((u >> 3) & (kC - 1)) >= valid) *reinterpret_cast<uint4*>(sm.stage[c % kStages].v + 16 * u) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async();
+            mbar_arrive(&sm.keys_ready[c & 1]);
+        };
+        if (kSums) {
+            for (int c = 0; c < chunks && !failed; ++c) {
+                if (c > 1 && !wait3(sm.done, c - 2)) break;  // the keys' buffer has been read
+                decay_keys(c);
+            }
+        } else {
+            if (chunks > 0) decay_keys(0);
+            for (int c = 0; c < chunks && !failed; ++c) {
+                // the state as an operand, and decayed over the chunk
+                if (c > 0 && !wait3(sm.done, c - 1)) break;
                 tc::fence_after_sync();
-                const float decay = decay_power(g, valid);
+                const float decay = decay_power(g, min(kC, end - begin - c * kC));
                 float down = 1.0f;
                 if constexpr (!kBf16) {
                     float most = 0.0f;
@@ -363,194 +467,169 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const ChunkCall
                         for (int e = 0; e < 32; ++e) most = fmaxf(most, fabsf(__uint_as_float(r[e])));
                     }
                     const int mine = static_cast<int>(__float_as_uint(most) >> 23);
-                    sm.most[0][side][row] = static_cast<uint16_t>(mine);
+                    sm.most_state[side][row] = static_cast<uint8_t>(mine);
                     mbar_arrive(&sm.most_ready[0]);
-                    if (!wait(&sm.most_ready[0], c & 1)) break;
-                    const float2 s = down_and_up(max(mine, static_cast<int>(sm.most[0][side ^ 1][row])));
-                    down = s.x;
-                    up = s.y;
+                    if (!wait(&sm.most_ready[0], c)) break;
+                    const int2 f = down_and_up(max(mine, static_cast<int>(sm.most_state[side ^ 1][row])));
+                    down = of_field(f.x);
+                    if (side == 0) sm.up[c % 3][row] = static_cast<uint8_t>(f.y);
                 }
 #pragma unroll 1
                 for (int b = 0; b < kHalf / 32; ++b) {
-                    uint32_t r[32], first[16], second[16];
+                    uint32_t r[32], operand[16];
                     tc::tmem_ld32(state_at + 32 * b, r);
                     tc::tmem_ld_wait();
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        float x = __uint_as_float(r[2 * e]), y = __uint_as_float(r[2 * e + 1]);
-                        r[2 * e] = __float_as_uint(x * decay);
-                        r[2 * e + 1] = __float_as_uint(y * decay);
-                        if constexpr (!kBf16) x *= down, y *= down;
-                        first[e] = pack_pair<kBf16>(x, y);
-                        const float2 f = unpack_pair<kBf16>(first[e]);
-                        second[e] = pack_pair<kBf16>(x - f.x, y - f.y);
+                        const F2 x = pair_of_words(r[2 * e], r[2 * e + 1]);
+                        operand[e] = pack_pair<kBf16>(kBf16 ? x : mul2(x, F2(down, down)));
+                        const float2 y = mul2(x, F2(decay, decay)).get();
+                        r[2 * e] = __float_as_uint(y.x);
+                        r[2 * e + 1] = __float_as_uint(y.y);
                     }
                     tc::tmem_st32(state_at + 32 * b, r);
-                    tc::tmem_st16(tmem + lanes + kFirstCol + (side * kHalf + 32 * b) / 2, first);
-                    tc::tmem_st16(tmem + lanes + kSecondCol + (side * kHalf + 32 * b) / 2, second);
+                    tc::tmem_st16(tmem + lanes + kOperandCol + (side * kHalf + 32 * b) / 2, operand);
                 }
                 tc::tmem_st_wait();
                 tc::fence_before_sync();
-                mbar_arrive(&sm.state_ready);
-                if (!wait(&sm.scores, c & 1)) break;  // the keys have been read, too
-                tc::fence_after_sync();
-            }
-            if (!wait(&sm.full[st], (c >> 1) & 1)) break;
-            // ---- decayed keys: the first numbers in the keys' place, the second beside them
-            {
-                unsigned char* const keys = sm.k[st];
-                unsigned char* const second = kSums ? sm.q[st] : sm.x;
-                constexpr int kEach = kC * D / 8 / kComputeThreads;
-#pragma unroll
-                for (int n = 0; n < kEach; ++n) {
-                    const int u = tid + n * kComputeThreads, j = (u >> 3) & (kC - 1);
-                    const float w = kSums ? (j < valid ? decay_power(g, end - 1 - t - j) : 0.0f) : (j < valid ? sm.power[valid - 1 - j] : 0.0f);
-                    const uint4 raw = *reinterpret_cast<const uint4*>(keys + 16 * u);
-                    const uint32_t in[4] = {raw.x, raw.y, raw.z, raw.w};
-                    uint32_t a[4], b[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 f = unpack_pair<kBf16>(in[e]);
-                        const float x = f.x * w, y = f.y * w;
-                        a[e] = pack_pair<kBf16>(x, y);
-                        const float2 h = unpack_pair<kBf16>(a[e]);
-                        b[e] = pack_pair<kBf16>(x - h.x, y - h.y);
-                    }
-                    *reinterpret_cast<uint4*>(keys + 16 * u) = make_uint4(a[0], a[1], a[2], a[3]);
-                    *reinterpret_cast<uint4*>(second + 16 * u) = make_uint4(b[0], b[1], b[2], b[3]);
-                }
-                fence_proxy_async();
-                mbar_arrive(&sm.keys_ready[st]);
-            }
-            if (kSums) continue;
-            // ---- P: row `row`, 64 columns
-            uint32_t p[32];
-            {
-                float most = 0.0f;
-                uint32_t s[2][32];
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const int j0 = 64 * side + 32 * b;
-                    if (j0 <= 32 * quad + 31) {  // a block with something on or below the diagonal
-                        tc::tmem_ld32(tmem + lanes + kScoreCol + j0, s[b]);
-                        tc::tmem_ld_wait();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const int n = row - j0 - e;
-                            const float x = n >= 0 ? __uint_as_float(s[b][e]) * sm.power[n & (kC - 1)] : 0.0f;
-                            if constexpr (!kBf16) most = fmaxf(most, fabsf(x));
-                            s[b][e] = __float_as_uint(x);
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) s[b][e] = 0u;
-                    }
-                }
-                tc::fence_before_sync();
-                mbar_arrive(&sm.scores_read);
-                float down = 1.0f;
-                if constexpr (!kBf16) {
-                    const int mine = static_cast<int>(__float_as_uint(most) >> 23);
-                    sm.most[1][side][row] = static_cast<uint16_t>(mine);
-                    mbar_arrive(&sm.most_ready[1]);
-                    if (!wait(&sm.most_ready[1], c & 1)) break;
-                    const float2 f = down_and_up(max(mine, static_cast<int>(sm.most[1][side ^ 1][row])));
-                    down = f.x;
-                    if (side == 0) sm.inside[row] = V.scale * f.y;
-                }
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    float x = __uint_as_float(s[e >> 4][2 * (e & 15)]), y = __uint_as_float(s[e >> 4][2 * (e & 15) + 1]);
-                    if constexpr (!kBf16) x *= down, y *= down;
-                    p[e] = pack_pair<kBf16>(x, y);
-                }
-            }
-            if (!wait(&sm.state_done, c & 1)) break;  // the second numbers of the keys have been read
-            {
-                unsigned char* const to = sm.x + side * (kC * 128) + row * 128;
-#pragma unroll
-                for (int u = 0; u < 8; ++u) *reinterpret_cast<uint4*>(to + ((u ^ (row & 7)) << 4)) = make_uint4(p[4 * u], p[4 * u + 1], p[4 * u + 2], p[4 * u + 3]);
-                fence_proxy_async();
-                mbar_arrive(&sm.p_ready);
-            }
-            if (!kBf16 && !wait(&sm.p_ready, c & 1)) break;  // sm.inside of all rows
-            // ---- the outputs: head dim `dim`, 64 tokens (heads of 64 dims, which are there twice: 32)
-            if (!wait(&sm.out_full, c & 1)) break;
-            tc::fence_after_sync();
-            constexpr int kBlocks = D == 128 ? 2 : 1;
-            const int i0 = D == 128 ? 64 * side : 64 * side + 32 * (quad >> 1);
-            uint16_t* const out = V.out + (static_cast<int64_t>(t) * V.v_heads + head) * D + dim;
-            const int64_t out_stride = static_cast<int64_t>(V.v_heads) * D;
-#pragma unroll 1
-            for (int b = 0; b < kBlocks; ++b) {
-                const int i1 = i0 + 32 * b;
-                uint32_t r[32], s[32];
-                tc::tmem_ld32(tmem + lanes + kOutCol + i1, r);
-                tc::tmem_ld32(tmem + lanes + kScoreCol + i1, s);
-                tc::tmem_ld_wait();
-                float zero = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    const float in = kBf16 ? V.scale : sm.inside[i1 + e];
-                    const float y = fmaf(__uint_as_float(r[e]), in, __uint_as_float(s[e]) * (sm.before[i1 + e] * up));
-                    zero = fmaf(y, 0.0f, zero);
-                    r[e] = __float_as_uint(y);
-                }
-                if (!(zero == 0.0f)) {
-#pragma unroll 1
-                    for (int e = 0; e < 32; ++e) {
-                        const int i = i1 + e;
-                        uint32_t word = 0;  // r[e], s[e] without an index into registers
-#pragma unroll
-                        for (int x = 0; x < 32; ++x)
-                            if (x == e) word = r[x];
-                        if ((word & 0x7F800000u) != 0x7F800000u || i >= valid) continue;
-                        uint32_t state_part = 0;
-#pragma unroll
-                        for (int x = 0; x < 32; ++x)
-                            if (x == e) state_part = s[x];
-                        const float in = kBf16 ? V.scale : sm.inside[i];
-                        const float y = fmaf(inside_again<kBf16>(sm.x, i, V.v + t * V.v_stride + head * D + dim, V.v_stride), in, __uint_as_float(state_part) * (sm.before[i] * up));
-#pragma unroll
-                        for (int x = 0; x < 32; ++x)
-                            if (x == e) r[x] = __float_as_uint(y);
-                    }
-                }
-                if (b == kBlocks - 1) {
-                    tc::fence_before_sync();
-                    mbar_arrive(&sm.out_read);
-                }
-#pragma unroll
-                for (int e = 0; e < 32; ++e)
-                    if (i1 + e < valid) out[(i1 + e) * out_stride] = f32_to_out<kBf16>(__uint_as_float(r[e]));
-                __syncwarp();
+                mbar_arrive(&sm.state_ready[c % 3]);
+                if (c + 1 < chunks) decay_keys(c + 1);  // their buffer's last reader was done before the state was
             }
         }
         // ---- what is left in tensor memory: the state behind the sequence, or the segment's sum
+        if (!failed && chunks > 0) wait3(sm.done, chunks - 1);
         if (!failed && (kSums ? chunks > 0 : last_segment)) {
-            if (kSums && !wait(&sm.state_done, 0)) {
-            } else {
-                tc::fence_after_sync();
-                float* const to = kSums ? sums : V.state_of(seq.to, head);
-                const float* const first = V.state_of(seq.from, head);
-                const float w = decay_power(g, P.segment);
+            tc::fence_after_sync();
+            float* const to = kSums ? sums : V.state_of(seq.to, head);
+            const float* const first = V.state_of(seq.from, head);
+            const float w = decay_power(g, P.segment);
 #pragma unroll 1
-                for (int b = 0; b < kHalf / 32; ++b) {
-                    uint32_t r[32];
-                    const int col = side * kHalf + 32 * b;
-                    tc::tmem_ld32(state_at + 32 * b, r);
-                    tc::tmem_ld_wait();
-                    if (row < D) {
+            for (int b = 0; b < kHalf / 32; ++b) {
+                uint32_t r[32];
+                const int col = side * kHalf + 32 * b;
+                tc::tmem_ld32(state_at + 32 * b, r);
+                tc::tmem_ld_wait();
+                if (row < D) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            float x = __uint_as_float(r[e]);
-                            if (kSums && unit.index == 0) x = fmaf(w, first[(col + e) * D + dim], x);
-                            to[(col + e) * D + dim] = x;
-                        }
+                    for (int e = 0; e < 32; ++e) {
+                        float x = __uint_as_float(r[e]);
+                        if (kSums && unit.index == 0) x = fmaf(w, first[(col + e) * D + dim], x);
+                        to[(col + e) * D + dim] = x;
                     }
-                    __syncwarp();
                 }
+                __syncwarp();
             }
+        }
+    } else if (!kSums && warp >= kLastWarps) {
+        // ---- score warps: rows 0 .. 63 of the scores, 32 columns a warp
+        const int quad = warp & 3, side = (warp - kLastWarps) >> 2, row = 32 * quad + lane, j0 = 32 * side;
+        for (int c = 0; c < chunks; ++c) {
+            if (!wait2(sm.scores, c)) break;
+            tc::fence_after_sync();
+            uint32_t s[32], p[16];
+            float most = 0.0f;
+            if (side <= quad) {  // a block with something on or below the diagonal
+                tc::tmem_ld32(tmem + (static_cast<uint32_t>(32 * quad) << 16) + kScoreCol + j0, s);
+                const int x0 = kC - 1 - row + j0, below = row - j0;  // columns 0 .. below are on or below the diagonal
+                const float2* const fade = reinterpret_cast<const float2*>(sm.fade[x0 & 1] + (x0 & ~1));
+                tc::tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    const float2 w = fade[e / 2];
+                    const float2 x = mul2(pair_of_words(s[e], s[e + 1]), F2(w.x, w.y)).get();
+                    // not a product with 0: a score of a later token need not be finite
+                    s[e] = e <= below ? __float_as_uint(x.x) : 0u;
+                    s[e + 1] = e + 1 <= below ? __float_as_uint(x.y) : 0u;
+                    if constexpr (!kBf16) most = fmaxf(most, fmaxf(fabsf(__uint_as_float(s[e])), fabsf(__uint_as_float(s[e + 1]))));
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) s[e] = 0u;
+            }
+            float down = 1.0f, up = 1.0f;
+            if constexpr (!kBf16) {
+                const int mine = static_cast<int>(__float_as_uint(most) >> 23);
+                sm.most_p[c & 1][side][row] = static_cast<uint8_t>(mine);
+                mbar_arrive(&sm.most_ready[1]);
+                if (!wait(&sm.most_ready[1], c)) break;
+                const int2 f = down_and_up(max(mine, static_cast<int>(sm.most_p[c & 1][side ^ 1][row])));
+                down = of_field(f.x);
+                up = of_field(f.y);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const F2 x = pair_of_words(s[2 * e], s[2 * e + 1]);
+                p[e] = pack_pair<kBf16>(kBf16 ? x : mul2(x, F2(down, down)));
+            }
+            if (c > 1 && !wait2(sm.out_read, c - 2)) break;  // nobody looks at P of the chunk before the last, and its scales, any more
+            if (!kBf16 && side == 0) sm.inside[c & 1][row] = V.scale * up;
+            unsigned char* const to = sm.p[c & 1] + row * 128;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) *reinterpret_cast<uint4*>(to + (((4 * side + u) ^ (row & 7)) << 4)) = make_uint4(p[4 * u], p[4 * u + 1], p[4 * u + 2], p[4 * u + 3]);
+            fence_proxy_async();
+            tc::fence_before_sync();
+            mbar_arrive(&sm.p_ready[c & 1]);
+        }
+    } else if (!kSums) {
+        // ---- row warps: head dim `dim`, 32 tokens (heads of 64 dims, which are there twice: 16), 16 at a time
+        const int quad = warp & 3, side = (warp - kStateWarps) >> 2, row = 32 * quad + lane, dim = row % D;
+        const uint32_t lanes = static_cast<uint32_t>(32 * quad) << 16;
+        constexpr int kTokens = 16, kBlocks = D == 128 ? 2 : 1;
+        const int first = D == 128 ? 32 * side : 32 * side + 16 * (quad >> 1);
+        for (int c = 0; c < chunks; ++c) {
+            const int64_t t = begin + c * kC;
+            const int valid = min(kC, end - static_cast<int>(t));
+            if (!wait3(sm.done, c)) break;
+            if (!kBf16 && (!wait3(sm.state_ready, c) || !wait2(sm.p_ready, c))) break;  // sm.up, sm.inside of all rows
+            if (c > 1 && !wait2(sm.out_free, c - 2)) break;
+            tc::fence_after_sync();
+            const float up = kBf16 ? 1.0f : of_field(sm.up[c % 3][row]);
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                const int i0 = first + kTokens * b;
+                uint32_t r[kTokens], s[kTokens];
+                tc::tmem_ld16(tmem + lanes + kInsideCol + (c & 1) * kC + i0, r);
+                tc::tmem_ld16(tmem + lanes + kBeforeCol + (c & 1) * kC + i0, s);
+                tc::tmem_ld_wait();
+                F2 zeros(0.0f, 0.0f);
+#pragma unroll
+                for (int e = 0; e < kTokens; e += 2) {
+                    const float2 in = kBf16 ? make_float2(V.scale, V.scale) : *reinterpret_cast<const float2*>(&sm.inside[c & 1][i0 + e]);
+                    const float2 before = *reinterpret_cast<const float2*>(&sm.before[i0 + e]);
+                    F2 part = mul2(pair_of_words(s[e], s[e + 1]), F2(before.x, before.y));
+                    if constexpr (!kBf16) part = mul2(part, F2(up, up));
+                    const F2 y = fma2(pair_of_words(r[e], r[e + 1]), F2(in.x, in.y), part);
+                    zeros = fma2(y, F2(0.0f, 0.0f), zeros);
+                    r[e] = __float_as_uint(y.get().x);
+                    r[e + 1] = __float_as_uint(y.get().y);
+                }
+                if (!(zeros.get().x + zeros.get().y == 0.0f)) {
+#pragma unroll 1
+                    for (int e = 0; e < kTokens; ++e) {
+                        const int i = i0 + e;
+                        uint32_t word = 0, part = 0;  // r[e], s[e] without an index into registers
+#pragma unroll
+                        for (int x = 0; x < kTokens; ++x)
+                            if (x == e) word = r[x], part = s[x];
+                        if ((word & 0x7F800000u) != 0x7F800000u || i >= valid) continue;
+                        const float in = kBf16 ? V.scale : sm.inside[c & 1][i];
+                        const float again = inside_again<kBf16>(sm.p[c & 1], i, V.v + t * V.v_stride + head * D + dim, V.v_stride);
+                        const float y = fmaf(again, in, __uint_as_float(part) * sm.before[i] * up);
+#pragma unroll
+                        for (int x = 0; x < kTokens; ++x)
+                            if (x == e) r[x] = __float_as_uint(y);
+                    }
+                }
+                __syncwarp();
+                if (b == kBlocks - 1) {
+                    tc::fence_before_sync();
+                    mbar_arrive(&sm.out_read[c & 1]);
+                }
+                uint32_t* const out = sm.out[c & 1] + i0 / 2 * D + dim;
+#pragma unroll
+                for (int e = 0; e < kTokens / 2; ++e) out[e * D] = pack_pair<kBf16>(pair_of_words(r[2 * e], r[2 * e + 1]));
+            }
+            mbar_arrive(&sm.out_ready[c & 1]);
         }
     }
     if (failed && lane == 0 && V.error_word != nullptr) atomicOr(V.error_word, KVB_ERR_WAIT_TIMEOUT);
@@ -589,12 +668,36 @@ int linear_segment(int tokens, int batch, int v_heads) {
 }
 int linear_units(int tokens, int batch, int segment) { return tokens / segment + batch; }
 
+namespace {
+
+// The driver's encoder of tensor maps; null where there is none.
+decltype(&cuTensorMapEncodeTiled) tensor_map_encoder() {
+    static const auto encoder = [] {
+        void* entry = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        const bool ok = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &entry, 12000, cudaEnableDefault, &found) == cudaSuccess && found == cudaDriverEntryPointSuccess;
+        return ok ? reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(entry) : nullptr;
+    }();
+    return encoder;
+}
+bool rows_map(CUtensorMap* map, const void* rows, bool bf16, int64_t width, int64_t tokens, int64_t stride) {
+    const auto encode = tensor_map_encoder();
+    const cuuint64_t size[2] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(tokens)}, pitch[1] = {static_cast<cuuint64_t>(stride) * 2};
+    const cuuint32_t box[2] = {64, kC}, step[2] = {1, 1};
+    return encode != nullptr && encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(rows), size, pitch, box, step,
+                                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace
+
 int linear_chunks(const LinearView& V, bool bf16, bool aligned, void* workspace, cudaStream_t stream) {
-    ChunkCall P;
+    ChunkCall P{};
     P.V = V;
     P.sums = workspace_base(workspace);
     P.segment = linear_segment(V.tokens, V.batch, V.v_heads);
-    P.aligned = aligned;
+    const int64_t qk_width = static_cast<int64_t>(V.v_heads) / V.share * V.head_dim, v_width = static_cast<int64_t>(V.v_heads) * V.head_dim;
+    P.aligned = aligned && rows_map(&P.q, V.q, bf16, qk_width, V.tokens, V.q_stride) && rows_map(&P.k, V.k, bf16, qk_width, V.tokens, V.k_stride) &&
+                rows_map(&P.v, V.v, bf16, v_width, V.tokens, V.v_stride);
     const int units = linear_units(V.tokens, V.batch, P.segment);
     if (V.head_dim == 128) return bf16 ? launch_chunks<128, true>(P, units, stream) : launch_chunks<128, false>(P, units, stream);
     return bf16 ? launch_chunks<64, true>(P, units, stream) : launch_chunks<64, false>(P, units, stream);

@@ -29,8 +29,9 @@ def _wanted(layer, q, k, v, scale, first):
 
     A term at a distance of n tokens has the decay's power n: exp is off by 2^-22 (two units in the last place), so its n-th power by n 2^-22, and the
     running product rounds n times; the chunked form's exponent n * log_decay, rounded, is off by n |log_decay| 2^-24 and meets 0 where it is large.
-    The products' 16-bit operands: scores are rounded to the type (half a step), keys and states are split into two numbers of the type that hold 16
-    bits together (bf16; 22 of fp16).  Sums in fp32: 2^-24 a term of what is summed, D terms of a product and 16 partial sums more."""
+    The products' 16-bit operands: scores, and for the outputs the states' elements, are rounded to the type (half a step: of a score what is left of
+    its sum, of a state's element at most the sum of the magnitudes that it came from); keys are split into two numbers of the type that
+    hold 16 bits together (bf16; 22 of fp16).  Sums in fp32: 2^-24 a term of what is summed, D terms of a product and 16 partial sums more."""
     import torch
 
     T, D = q.shape[0], q.shape[2]
@@ -56,8 +57,8 @@ def _wanted(layer, q, k, v, scale, first):
     split = 2.0 ** -16 if layer.dtype == torch.bfloat16 else 2.0 ** -21
     sums = (D + 16) * 2.0 ** -24
     mag = q.abs() @ k.abs().transpose(1, 2)
-    out_off = ((seen * (power(gap) * (u * s.abs() + (split + 2 * sums) * mag) + off(gap) * mag)) @ v.abs()
-               + (power(n[:, None] + 1) * (split + sums) + off(n[:, None] + 1)) * (q.abs() @ first.abs())) * scale
+    out_off = ((seen * (power(gap) * (u * s.abs() + (u + split + 2 * sums) * mag) + off(gap) * mag)) @ v.abs()
+               + (power(n[:, None] + 1) * (u + split + sums) + off(n[:, None] + 1)) * (q.abs() @ first.abs())) * scale
     # what stays of a state was summed once a chunk or token: roundings of what it held, decayed
     held = (k.abs() * power(T - 1 - n[:, None])).transpose(1, 2) @ v.abs() + power(torch.full_like(g, T)) * first.abs()
     steps = 1 / (1 - torch.exp(g)).clamp_min(1.0 / max(T, 1))  # tokens that a state remembers
@@ -92,7 +93,14 @@ def _i32(x):
 
 
 def _close(got, want, off, what):
+    """Within the worst case, value by value; outputs also in the mean square: roundings of three kinds (the output's; scores' and states' beside each other), each
+    uniform over at most half a step and independent: sqrt(2 / 3) of half a step together where the two parts do not cancel, 1.2 allowed."""
+    import torch
+
     err = (got.double() - want).abs()
+    if got.dtype != torch.float32 and want.numel() > 4096:
+        half = torch.finfo(got.dtype).eps / 2
+        assert float(err.square().sum().sqrt()) <= 1.2 * half * float(want.square().sum().sqrt()) + 2.0 ** -25 * want.numel() ** 0.5, what
     assert bool((err <= off).all()), f"{what}: {int((~(err <= off)).sum())} values off, by up to {float((err / off.clamp_min(1e-300)).max()):.2f} of the tolerance"
 
 
@@ -145,6 +153,42 @@ def test_chunk(dtype, qk, vh, D, lengths):
         o, oo, s, so = _wanted(layer, q[rows], k[rows], v[rows], D ** -0.5, before[reads[b]])
         _close(out[rows], o, oo, f"out {b}")
         _close(layer.state[writes[b]], s, so, f"state {b}")
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lengths", [[193], [256], [320, 1, 641], [1100]])
+def test_chunk_with_many_heads(dtype, D, lengths):
+    """So many heads that a sequence is one segment of several chunks."""
+    import torch
+
+    n, tokens, vh = len(lengths), sum(lengths), 80
+    layer = _layer(40, vh, D, n, dtype)
+    before = _fill(layer, tokens)
+    q, k, v = _inputs(40, vh, D, tokens, dtype, tokens)
+    offsets = [sum(lengths[:b]) for b in range(n + 1)]
+    slots = _i32(list(range(n)))
+    out = layer.chunk(q, k, v, _i32(offsets), D ** -0.5, slots, slots)
+    assert layer.errors() == 0
+    for b in range(n):
+        rows = slice(offsets[b], offsets[b + 1])
+        o, oo, s, so = _wanted(layer, q[rows], k[rows], v[rows], D ** -0.5, before[b])
+        _close(out[rows], o, oo, f"out {b}")
+        _close(layer.state[b], s, so, f"state {b}")
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+def test_outputs_at_any_boundary(shift):
+    import torch
+
+    T = 300
+    layer = _layer(80, 80, 64, 2, "bf16")
+    q, k, v = _inputs(80, 80, 64, T, "bf16", 7)
+    buf = torch.full((T * 80 * 64 + 16,), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = buf[shift + 8:shift + 8 + T * 80 * 64].view(T, 80, 64)
+    layer.chunk(q, k, v, _i32([0, T]), 0.1, _i32([0]), _i32([1]), out=out)
+    assert torch.equal(out, layer.chunk(q, k, v, _i32([0, T]), 0.1, _i32([0]), _i32([1])))
+    assert bool((buf[:shift + 8] == 7).all()) and bool((buf[shift + 8 + T * 80 * 64:] == 7).all()) and layer.errors() == 0
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
