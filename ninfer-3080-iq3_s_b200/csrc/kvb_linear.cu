@@ -39,8 +39,8 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(LinearView L) {
     const int seq = blockIdx.z, head = blockIdx.y, col0 = blockIdx.x * kCols, tid = threadIdx.x;
     const Sequence s = L.sequence(seq);
     if (!s.valid) return;
-    float lambda;
-    if (!L.decay_of(head, &lambda)) return;
+    const float g = L.log_decay[head], lambda = expf(g);
+    if (!L.decay_fits(g)) return;
     const int vec = tid % kVecs, group = tid / kVecs;
     const float* from = L.state_of(s.from, head) + col0 + 4 * vec;
     float* to = L.state_of(s.to, head) + col0 + 4 * vec;

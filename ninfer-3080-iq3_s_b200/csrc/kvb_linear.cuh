@@ -39,22 +39,22 @@ struct LinearView {
         s.end = offsets != nullptr ? offsets[seq + 1] : seq + 1;
         s.from = reads[seq];
         s.to = writes[seq];
-        const bool rows = s.begin >= 0 && s.end >= s.begin && s.end <= tokens;
-        const bool pool = s.from >= 0 && s.from < slots && s.to >= 0 && s.to < slots;
         bool shared = false;
         for (int i = threadIdx.x; i < batch; i += blockDim.x)
             if (i != seq) shared = shared || writes[i] == s.to || reads[i] == s.to || writes[i] == s.from;
-        shared = __syncthreads_or(shared) != 0;
-        if (!rows) flag(KVB_ERR_POSITIONS);
-        if (!pool || shared) flag(KVB_ERR_SLOT);
-        s.valid = rows && pool && !shared;
+        s.valid = judge(s, __syncthreads_or(shared) != 0);
         return s;
     }
-    // exp(log_decay): 0 .. 1; a head with another one is refused.
-    __device__ __forceinline__ bool decay_of(int head, float* lambda) const {
-        const float g = log_decay[head];
-        *lambda = expf(g);
-        if (g <= 0.0f) return true;
+    __device__ __forceinline__ bool judge(const Sequence& s, bool shared) const {
+        const bool rows = s.begin >= 0 && s.end >= s.begin && s.end <= tokens;
+        const bool pool = s.from >= 0 && s.from < slots && s.to >= 0 && s.to < slots;
+        if (!rows) flag(KVB_ERR_POSITIONS);
+        if (!pool || shared) flag(KVB_ERR_SLOT);
+        return rows && pool && !shared;
+    }
+    // exp(log_decay) is 0 .. 1; a head with another one is refused.
+    __device__ __forceinline__ bool decay_fits(float log_decay_of_head) const {
+        if (log_decay_of_head <= 0.0f) return true;
         flag(KVB_ERR_GEOMETRY);
         return false;
     }

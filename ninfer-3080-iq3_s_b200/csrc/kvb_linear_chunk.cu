@@ -14,13 +14,14 @@
 //
 // Warps by role, so that a chunk's steps run beside its neighbours':
 //   state warps   the state as an operand (then decayed over the chunk), decayed keys of the next chunk
-//   score warps   P, a chunk ahead
+//   score warps   P, up to two chunks ahead
 //   row warps     outputs
-//   an MMA warp   P V and the next chunk's scores while the state becomes an operand; then S += K'^T V and the outputs' part from before
+//   an MMA warp   S += K'^T V, and the outputs' part from before
+//   another       P V, and scores two chunks ahead
 //   a load warp   tiles by TMA, into three stages (16-byte copies by the lanes filled the SM's load queue, where everybody's shared-memory accesses
-//                 and arrivals waited behind them: 5,400 cycles a chunk)
-//   store warps   outputs, 16 bytes a lane (two bytes a lane from the row warps held those up for 4,000 cycles a chunk, most of it in the fence before
-//                 the next P, which waits for the thread's stores)
+//                 and arrivals waited behind them)
+//   a store warp  outputs, 16 bytes a lane (two bytes a lane from the row warps held those up for 4,000 cycles a chunk, most of it in the fence before
+//                 their next accesses for the MMAs, which waits for the thread's stores)
 // The loop that cannot be shortened is state -> operand -> two products -> state.
 //
 // A sequence is split into segments where there are fewer heads and sequences than SMs: a first launch sums up each segment alone
@@ -39,8 +40,8 @@ namespace {
 constexpr int kC = kLinearChunk;  // tokens of a chunk
 constexpr int kStages = 3;
 constexpr int kStateWarps = 8, kRowWarps = 8;
-// the last eight: warp 0, 1, 4, 5 of them P (rows 0 .. 63 of tensor memory are a warp's by its number mod 4), 2 MMAs, 3 loads, 6, 7 stores of even and odd chunks
-constexpr int kLastWarps = kStateWarps + kRowWarps, kMmaWarp = kLastWarps + 2, kLoadWarp = kLastWarps + 3, kStoreWarp = kLastWarps + 6;
+// the last eight: warps 0, 1, 4, 5 of them P (rows 0 .. 63 of tensor memory are a warp's by its number mod 4)
+constexpr int kLastWarps = kStateWarps + kRowWarps, kStateMmaWarp = kLastWarps + 2, kLoadWarp = kLastWarps + 3, kRowMmaWarp = kLastWarps + 6, kStoreWarp = kLastWarps + 7;
 constexpr int kStateThreads = kStateWarps * 32, kRowThreads = kRowWarps * 32, kScoreThreads = 128;
 constexpr int kChunkThreads = (kLastWarps + 8) * 32;  // 24 warps: six to a scheduler, 80 registers a thread
 constexpr uint32_t kTmemCols = 512;
@@ -59,8 +60,8 @@ template <int D> struct LinearSmem {
     float inside[2][kC];                   // scale times what P's row i was scaled down by (fp16)
     uint8_t up[3][128];                    // exponent field of what a row of the state was scaled down by (fp16)
     uint8_t most_state[2][128], most_p[2][2][kC];  // exponents of the largest magnitudes of a row, one a column half (fp16)
-    // chunk c has the one of c mod their number; `done`: all products of a chunk
-    uint64_t full[kStages], done[kStages], state_ready[3], scores[2], p_ready[2], keys_ready[2], out_read[2], out_ready[2], out_free[2], most_ready[2], drained;
+    // chunk c has the one of c mod their number; done: the state's products of a chunk; rows_done: P V of chunk c - 2 and the scores of chunk c
+    uint64_t full[kStages], done[kStages], rows_done[kStages], state_ready[3], p_ready[2], keys_ready[2], out_read[2], out_ready[2], out_free[2], most_ready[2], loaded, drained[2];
     uint32_t tmem_base;
     int abort_flag;
     int unit[3];
@@ -74,39 +75,63 @@ struct ChunkCall {
     bool aligned;  // rows of q, k, v keep to 16 bytes: the maps are there
 };
 
-// Sequence and segment of the call's unit `unit`, found by one warp; the same for all threads afterwards.  seq = batch: none.
+// Which sequence and segment a unit is, and the checks of LinearView::sequence(), for the whole CTA: everything is asked of global memory at once,
+// one latency instead of one after another.  `scratch`: 3 kMostSequences + 1 words of shared memory.
 struct Unit {
-    int seq, index, count;  // segment `index` of `count`
+    int index, count;  // segment `index` of `count`; count = 0: nothing to do
+    Sequence seq;
+    float g;           // log_decay of the head
 };
-__device__ __forceinline__ int segments_of(const ChunkCall& P, int seq) {
-    const int begin = P.V.offsets[seq], end = P.V.offsets[seq + 1];
-    const int64_t length = static_cast<int64_t>(end) - begin;
-    return length <= 0 || length > P.V.tokens ? 1 : static_cast<int>((length + P.segment - 1) / P.segment);
-}
-__device__ __forceinline__ Unit unit_of(const ChunkCall& P, int unit, int (&shared)[3]) {
-    if (threadIdx.x < 32) {
+__device__ __forceinline__ Unit unit_of(const ChunkCall& P, int unit, int head, int32_t* scratch, int (&found)[3]) {
+    const LinearView& V = P.V;
+    const int tid = threadIdx.x, lane = tid & 31;
+    int32_t *const offsets = scratch, *const reads = scratch + kMostSequences + 1, *const writes = reads + kMostSequences;
+    static_assert(kMostSequences < kChunkThreads, "a thread a sequence");
+    Unit u;
+    u.g = V.log_decay[head];
+    if (tid <= V.batch) offsets[tid] = V.offsets[tid];
+    if (tid < V.batch) {
+        reads[tid] = V.reads[tid];
+        writes[tid] = V.writes[tid];
+    }
+    __syncthreads();
+    if (tid < 32) {
         int base = 0;
-        bool found = false;
-        for (int s0 = 0; s0 < P.V.batch; s0 += 32) {
-            const int seq = s0 + static_cast<int>(threadIdx.x);
-            const int count = seq < P.V.batch ? segments_of(P, seq) : 0;
+        bool any = false;
+        for (int s0 = 0; s0 < V.batch; s0 += 32) {
+            const int seq = s0 + lane;
+            int count = 0;
+            if (seq < V.batch) {
+                const int64_t length = static_cast<int64_t>(offsets[seq + 1]) - offsets[seq];
+                count = length <= 0 || length > V.tokens ? 1 : static_cast<int>((length + P.segment - 1) / P.segment);
+            }
             int sum = count;  // inclusive
 #pragma unroll
             for (int step = 1; step < 32; step <<= 1) {
                 const int up = __shfl_up_sync(0xffffffffu, sum, step);
-                if (static_cast<int>(threadIdx.x) >= step) sum += up;
+                if (lane >= step) sum += up;
             }
             const bool mine = unit >= base + sum - count && unit < base + sum;
-            if (mine) shared[0] = seq, shared[1] = unit - (base + sum - count), shared[2] = count;
-            found = __any_sync(0xffffffffu, mine) || found;
+            if (mine) found[0] = seq, found[1] = unit - (base + sum - count), found[2] = count;
+            any = __any_sync(0xffffffffu, mine) || any;
             base += __shfl_sync(0xffffffffu, sum, 31);
         }
-        if (!found && threadIdx.x == 0) shared[0] = P.V.batch, shared[1] = shared[2] = 0;
+        if (!any && lane == 0) found[0] = found[1] = found[2] = 0;
         // sequences that overlap have more segments than the grid has units: what is left out is reported
-        if (unit == 0 && base > static_cast<int>(gridDim.x)) P.V.flag(KVB_ERR_POSITIONS);
+        if (unit == 0 && base > static_cast<int>(gridDim.y)) V.flag(KVB_ERR_POSITIONS);
     }
     __syncthreads();
-    return Unit{shared[0], shared[1], shared[2]};
+    const int seq = found[0];
+    u.index = found[1];
+    u.count = found[2];
+    u.seq.begin = offsets[seq];
+    u.seq.end = offsets[seq + 1];
+    u.seq.from = reads[seq];
+    u.seq.to = writes[seq];
+    const bool other = tid < V.batch && tid != seq;
+    const bool shared = __syncthreads_or(other && (writes[tid] == u.seq.to || reads[tid] == u.seq.to || writes[tid] == u.seq.from)) != 0;
+    u.seq.valid = u.count > 0 && V.judge(u.seq, shared);
+    return u;
 }
 
 // exp(g n): 1 at n = 0, whatever g is.
@@ -145,6 +170,7 @@ __device__ __forceinline__ int2 down_and_up(int field) {
 }
 
 // A box of a tensor map into shared memory, from `row` and the first dim `x` on (a multiple of 64).
+__device__ __forceinline__ void prefetch_map(const CUtensorMap& map) { asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map)) : "memory"); }
 __device__ __forceinline__ void tma_load(unsigned char* dst, const CUtensorMap& map, int x, int row, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
                  "l"(reinterpret_cast<uint64_t>(&map)), "r"(x), "r"(row), "r"(smem_u32(bar))
@@ -184,40 +210,43 @@ template <int D, bool kBf16, bool kSums>
 __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_constant__ ChunkCall P) {
     using Smem = LinearSmem<D>;
     constexpr int kHalf = D / 2;  // columns of the state a state warp has
-    constexpr uint32_t kStateCol = 0, kOperandCol = D, kScoreCol = D + D / 2, kBeforeCol = kScoreCol + kC, kInsideCol = kBeforeCol + 2 * kC;
-    static_assert(kInsideCol + 2 * kC <= kTmemCols, "tensor memory");
+    constexpr uint32_t kStateCol = 0, kOperandCol = D, kScoreCol = D + D / 2, kBeforeCol = kScoreCol + 2 * kC, kInsideCol = kBeforeCol + 2 * kC;
+    static_assert(kInsideCol + kC <= kTmemCols, "tensor memory");
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
     grid_dependency_wait();
     launch_dependents();
     const LinearView& V = P.V;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = blockIdx.y;
-    const Unit unit = unit_of(P, blockIdx.x, sm.unit);
-    if (unit.seq >= V.batch) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = blockIdx.x;
+    if (warp == kLoadWarp && lane == 0 && P.aligned) {
+        if (!kSums) prefetch_map(P.q);
+        prefetch_map(P.k);
+        prefetch_map(P.v);
+    }
+    const Unit unit = unit_of(P, blockIdx.y, head, reinterpret_cast<int32_t*>(sm.out), sm.unit);
+    const Sequence& seq = unit.seq;
     if (kSums && unit.count == 1) return;
-    const Sequence seq = V.sequence(unit.seq);
-    float lambda;
-    if (!seq.valid || !V.decay_of(head, &lambda)) return;
+    if (!seq.valid || !V.decay_fits(unit.g)) return;
     if ((smem_u32(smem_raw) & 1023u) != 0) {  // the swizzle needs it; the launch asks for nothing beside it
         V.flag(KVB_ERR_GEOMETRY);
         return;
     }
-    const float g = V.log_decay[head];
+    const float g = unit.g;
     const bool last_segment = unit.index == unit.count - 1;
     const int begin = seq.begin + unit.index * P.segment, end = last_segment ? seq.end : begin + P.segment;
     const int chunks = kSums && last_segment ? 0 : (end - begin + kC - 1) / kC;
-    float* const sums = P.sums + (static_cast<int64_t>(blockIdx.x) * V.v_heads + head) * D * D;  // this segment's; earlier ones lie in front
+    float* const sums = P.sums + (static_cast<int64_t>(blockIdx.y) * V.v_heads + head) * D * D;  // this segment's; earlier ones lie in front
     const int64_t sums_step = static_cast<int64_t>(V.v_heads) * D * D;
 
-    if (warp == kMmaWarp) tc::tmem_alloc(&sm.tmem_base, kTmemCols);
+    if (warp == kStateMmaWarp) tc::tmem_alloc(&sm.tmem_base, kTmemCols);
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&sm.full[s], 1);
             mbar_init(&sm.done[s], 1);
+            mbar_init(&sm.rows_done[s], 1);
             mbar_init(&sm.state_ready[s], kStateThreads);
         }
         for (int s = 0; s < 2; ++s) {
-            mbar_init(&sm.scores[s], 1);
             mbar_init(&sm.p_ready[s], kScoreThreads);
             mbar_init(&sm.keys_ready[s], kStateThreads);
             mbar_init(&sm.out_read[s], kRowThreads);
@@ -226,7 +255,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
         }
         mbar_init(&sm.most_ready[0], kStateThreads);
         mbar_init(&sm.most_ready[1], kScoreThreads);
-        mbar_init(&sm.drained, 1);
+        mbar_init(&sm.loaded, kStateThreads + kRowThreads);
+        mbar_init(&sm.drained[0], 1);
+        mbar_init(&sm.drained[1], 1);
         mbar_fence_init();
         sm.abort_flag = 0;
     }
@@ -247,6 +278,49 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
     auto wait2 = [&](uint64_t (&bars)[2], int c) { return wait(&bars[c & 1], c >> 1); };
     auto wait3 = [&](uint64_t (&bars)[3], int c) { return wait(&bars[c % 3], c / 3); };
 
+    if (warp < kLastWarps && (!kSums || last_segment)) {
+        // ---- the state before the segment, a quarter of the columns a warp: from the pool, or the sums of the segments before
+        const int quad = warp & 3, row = 32 * quad + lane, dim = row % D;
+        constexpr int kEach = D / 4;
+        const int col = (warp >> 2) * kEach;
+        const float* from = V.state_of(seq.from, head);
+        if (!kSums && unit.count > 1 && unit.index == 0) from = sums + (unit.count - 1) * sums_step;
+#pragma unroll 1
+        for (int b = 0; b < kEach; b += 16) {
+            const int at = (col + b) * D + dim;
+            uint32_t r[16];
+            if (kSums || unit.index == 0) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(from[at + e * D]);
+            } else {
+                float f[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) f[e] = 0.0f;
+#pragma unroll 2
+                for (int s = 0; s < unit.index; ++s) {
+                    const float* const sum = sums - (unit.index - s) * sums_step + at;
+                    const float w = decay_power(g, (unit.index - 1 - s) * P.segment);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) f[e] = fmaf(w, sum[e * D], f[e]);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(f[e]);
+            }
+            if (kSums) {  // the last segment's place keeps the state for the second launch, which may write over it
+                if (row < D) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) sums[at + e * D] = __uint_as_float(r[e]);
+                }
+            } else {
+                tc::tmem_st16(tmem + (static_cast<uint32_t>(32 * quad) << 16) + kStateCol + col + b, r);
+            }
+        }
+        if (!kSums) {
+            tc::tmem_st_wait();
+            tc::fence_before_sync();
+            mbar_arrive(&sm.loaded);
+        }
+    }
     if (warp == kLoadWarp) {
         // ---- loads: chunk c into stage c % 3.  Rows behind a sequence's last come with it, whatever they hold: see there.
         const int qk_head = head / V.share;
@@ -254,7 +328,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
             const int stage = c % kStages;
             typename Smem::Stage& st = sm.stage[stage];
             const int64_t t = begin + c * kC;
-            if (c >= kStages && !wait3(sm.done, c - kStages)) break;
+            // the products of the stage's chunk before: the state's, its P V
+            if (c >= kStages && (!wait3(sm.done, c - kStages) || (!kSums && !wait3(sm.rows_done, c - kStages + 2)))) break;
             if (P.aligned) {
                 if (lane == 0) {
                     mbar_expect_tx(&sm.full[stage], (kSums ? 2 : 3) * Smem::kTileBytes);
@@ -276,11 +351,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
         // no copy lands in shared memory that is no longer this CTA's
         if (failed && P.aligned)
             for (int c = max(0, chunks - kStages); c < chunks; ++c) mbar_wait_bounded(&sm.full[c % kStages], (c / kStages) & 1);
-    } else if (warp == kStoreWarp || warp == kStoreWarp + 1) {
-        // ---- stores: outputs of even chunks, of odd ones
+    } else if (warp == kStoreWarp) {
+        // ---- stores
         const bool wide = (reinterpret_cast<uintptr_t>(V.out) & 15u) == 0;
         const int64_t out_stride = static_cast<int64_t>(V.v_heads) * D;
-        for (int c = warp - kStoreWarp; !kSums && c < chunks; c += 2) {
+        for (int c = 0; !kSums && c < chunks; ++c) {
             const int64_t t = begin + c * kC;
             const int valid = min(kC, end - static_cast<int>(t));
             if (!wait2(sm.out_ready, c)) break;
@@ -313,61 +388,68 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.out_free[c & 1]);
         }
-    } else if (warp == kMmaWarp) {
-        // ---- MMAs, issued by one thread
+    } else if (warp == kStateMmaWarp || warp == kRowMmaWarp) {
+        // ---- MMAs, issued by one thread of a warp
         // MN-major: the next 64 head dims half a tile further (heads of 64 dims: the same ones again), the next 8 tokens 1024 bytes
         constexpr uint32_t kScores = idesc_16<kBf16>(128, kC, false, false), kState = idesc_16<kBf16>(128, D, true, true), kOut = idesc_16<kBf16>(128, kC, true, false);
         auto rows_desc = [&](const unsigned char* tile) { return tc::smem_desc(smem_u32(tile), 16, 1024); };
         auto dims_desc = [&](const unsigned char* tile) { return tc::smem_desc(smem_u32(tile), D == 128 ? kC * 128 : 0, 1024); };
+        auto keys_desc = [&](const unsigned char* tile) { return tc::smem_desc(smem_u32(tile), kC * 128, 1024); };
         auto k_major = [](uint64_t desc, int step) { return tc::desc_at(desc, (step >> 2) * (kC * 128) + (step & 3) * 32); };  // 16 of the K dims further
-        auto issue_scores = [&](int c) {
-            const typename Smem::Stage& st = sm.stage[c % kStages];
-            if (!wait3(sm.full, c)) return;
-            tc::fence_after_sync();
-            if (tc::elect_one()) {
-                const uint64_t a = tc::desc_here(rows_desc(st.q)), b = tc::desc_here(rows_desc(st.k));
-#pragma unroll
-                for (int s = 0; s < D / 16; ++s) tc::mma_f16_ss(tmem + kScoreCol, k_major(a, s), k_major(b, s), kScores, s > 0);
-                tc::commit(&sm.scores[c & 1]);
-            }
-            __syncwarp();
-        };
-        if (!kSums && chunks > 0) issue_scores(0);
-        for (int c = 0; c < chunks && !failed; ++c) {
-            const typename Smem::Stage& st = sm.stage[c % kStages];
-            if (!wait2(sm.keys_ready, c)) break;
-            if (!kSums) {  // beside the state's way into an operand: what does not need it
-                if (!wait2(sm.p_ready, c) || (c > 1 && !wait2(sm.out_read, c - 2))) break;
+        if (warp == kStateMmaWarp) {
+            for (int c = 0; c < chunks; ++c) {
+                const typename Smem::Stage& st = sm.stage[c % kStages];
+                if (!wait2(sm.keys_ready, c)) break;
+                // what is left of the outputs before the last in tensor memory has been read
+                if (!kSums && (!wait3(sm.state_ready, c) || (c > 1 && !wait2(sm.out_read, c - 2)))) break;
                 tc::fence_after_sync();
                 if (tc::elect_one()) {
-                    const uint64_t a = tc::desc_here(dims_desc(st.v)), b = tc::desc_here(rows_desc(sm.p[c & 1]));
+                    const uint64_t a = dims_desc(st.v), b = keys_desc(st.k), b2 = keys_desc(sm.second[c & 1]);
 #pragma unroll
-                    for (int s = 0; s < kC / 16; ++s) tc::mma_f16_ss(tmem + kInsideCol + (c & 1) * kC, tc::desc_at(a, s * 2048), k_major(b, s), kOut, s > 0);
+                    for (int s = 0; s < kC / 16; ++s) tc::mma_f16_ss(tmem + kStateCol, tc::desc_at(a, s * 2048), tc::desc_at(b, s * 2048), kState, !kSums || c > 0 || s > 0);
+#pragma unroll
+                    for (int s = 0; s < kC / 16; ++s) tc::mma_f16_ss(tmem + kStateCol, tc::desc_at(a, s * 2048), tc::desc_at(b2, s * 2048), kState, true);
+                    if (!kSums) {
+                        const uint64_t q = rows_desc(st.q);
+#pragma unroll
+                        for (int s = 0; s < D / 16; ++s) tc::mma_f16_ts(tmem + kBeforeCol + (c & 1) * kC, tmem + kOperandCol + 8 * s, k_major(q, s), kScores, s > 0);
+                    }
+                    tc::commit(&sm.done[c % 3]);
                 }
                 __syncwarp();
-                if (c + 1 < chunks) issue_scores(c + 1);
-                if (!wait3(sm.state_ready, c)) break;
             }
-            tc::fence_after_sync();
-            if (tc::elect_one()) {
-                const uint64_t a = tc::desc_here(dims_desc(st.v)), b = tc::desc_here(tc::smem_desc(smem_u32(st.k), kC * 128, 1024)), b2 = tc::desc_here(tc::smem_desc(smem_u32(sm.second[c & 1]), kC * 128, 1024));
+        } else if (!kSums) {
+            for (int n = 0; n < chunks + 2; ++n) {  // P V of chunk n - 2, scores of chunk n
+                const int c = n - 2;
+                if (c >= 0) {
+                    if (!wait2(sm.keys_ready, c) || !wait2(sm.p_ready, c) || (c > 0 && !wait2(sm.out_read, c - 1))) break;  // keys: values behind the last are zeros
+                    tc::fence_after_sync();
+                    if (tc::elect_one()) {
+                        const uint64_t a = dims_desc(sm.stage[c % kStages].v), b = rows_desc(sm.p[c & 1]);
 #pragma unroll
-                for (int s = 0; s < kC / 16; ++s) tc::mma_f16_ss(tmem + kStateCol, tc::desc_at(a, s * 2048), tc::desc_at(b, s * 2048), kState, !kSums || c > 0 || s > 0);
-#pragma unroll
-                for (int s = 0; s < kC / 16; ++s) tc::mma_f16_ss(tmem + kStateCol, tc::desc_at(a, s * 2048), tc::desc_at(b2, s * 2048), kState, true);
-                if (!kSums) {
-                    const uint64_t q = tc::desc_here(rows_desc(st.q));
-#pragma unroll
-                    for (int s = 0; s < D / 16; ++s) tc::mma_f16_ts(tmem + kBeforeCol + (c & 1) * kC, tmem + kOperandCol + 8 * s, k_major(q, s), kScores, s > 0);
+                        for (int s = 0; s < kC / 16; ++s) tc::mma_f16_ss(tmem + kInsideCol, tc::desc_at(a, s * 2048), k_major(b, s), kOut, s > 0);
+                    }
+                    __syncwarp();
                 }
-                tc::commit(&sm.done[c % 3]);
+                if (n < chunks) {
+                    if (!wait3(sm.full, n)) break;
+                    tc::fence_after_sync();
+                    if (tc::elect_one()) {
+                        const uint64_t a = rows_desc(sm.stage[n % kStages].q), b = rows_desc(sm.stage[n % kStages].k);
+#pragma unroll
+                        for (int s = 0; s < D / 16; ++s) tc::mma_f16_ss(tmem + kScoreCol + (n & 1) * kC, k_major(a, s), k_major(b, s), kScores, s > 0);
+                    }
+                    __syncwarp();
+                }
+                if (tc::elect_one()) tc::commit(&sm.rows_done[n % 3]);
+                __syncwarp();
             }
-            __syncwarp();
         }
         if (failed) {  // nothing is freed under MMAs that still run
-            if (tc::elect_one()) tc::commit(&sm.drained);
+            uint64_t* const drained = &sm.drained[warp == kRowMmaWarp];
+            if (tc::elect_one()) tc::commit(drained);
             __syncwarp();
-            mbar_wait_bounded(&sm.drained, 0);
+            mbar_wait_bounded(drained, 0);
         }
     } else if (warp < kStateWarps) {
         // ---- state warps: rows 32 (warp % 4) + lane of S^T, columns by warp / 4
@@ -375,46 +457,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
         const uint32_t lanes = static_cast<uint32_t>(32 * quad) << 16;
         const uint32_t state_at = tmem + lanes + kStateCol + side * kHalf;
 
-        if (!kSums || last_segment) {
-            // the state before the segment: from the pool, or the sums of the segments before
-            const float* from = V.state_of(seq.from, head);
-            if (!kSums && unit.count > 1 && unit.index == 0) from = sums + (unit.count - 1) * sums_step;
-#pragma unroll 1
-            for (int b = 0; b < kHalf / 32; ++b) {
-                uint32_t r[32];
-                const int col = side * kHalf + 32 * b;
-                if (kSums || unit.index == 0) {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(from[(col + e) * D + dim]);
-                } else {
-                    float f[32];
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) f[e] = 0.0f;
-#pragma unroll 1
-                    for (int s = 0; s < unit.index; ++s) {
-                        const float* sum = sums - (unit.index - s) * sums_step;
-                        const float w = decay_power(g, (unit.index - 1 - s) * P.segment);
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) f[e] = fmaf(w, sum[(col + e) * D + dim], f[e]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(f[e]);
-                }
-                if (kSums) {  // the last segment's place keeps the state for the second launch, which may write over it
-                    if (row < D) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) sums[(col + e) * D + dim] = __uint_as_float(r[e]);
-                    }
-                } else {
-                    tc::tmem_st32(state_at + 32 * b, r);
-                }
-            }
-            tc::tmem_st_wait();
-        }
         // decayed keys of chunk c, two numbers each
         auto decay_keys = [&](int c) {
             if (!wait3(sm.full, c)) return;
-            if (!kSums && !wait2(sm.scores, c)) return;  // the keys themselves have been read
+            if (!kSums && !wait3(sm.rows_done, c)) return;  // the keys themselves have been read
             const int t = begin + c * kC, valid = min(kC, end - t);
             unsigned char* const keys = sm.stage[c % kStages].k;
             unsigned char* const second = sm.second[c & 1];
@@ -450,6 +496,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
             }
         } else {
             if (chunks > 0) decay_keys(0);
+            wait(&sm.loaded, 0);
+            tc::fence_after_sync();
             for (int c = 0; c < chunks && !failed; ++c) {
                 // the state as an operand, and decayed over the chunk
                 if (c > 0 && !wait3(sm.done, c - 1)) break;
@@ -501,21 +549,22 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
         if (!failed && (kSums ? chunks > 0 : last_segment)) {
             tc::fence_after_sync();
             float* const to = kSums ? sums : V.state_of(seq.to, head);
-            const float* const first = V.state_of(seq.from, head);
             const float w = decay_power(g, P.segment);
 #pragma unroll 1
-            for (int b = 0; b < kHalf / 32; ++b) {
-                uint32_t r[32];
-                const int col = side * kHalf + 32 * b;
-                tc::tmem_ld32(state_at + 32 * b, r);
+            for (int b = 0; b < kHalf; b += 16) {
+                const int at = (side * kHalf + b) * D + dim;
+                uint32_t r[16];
+                float first[16];  // asked for ahead of the stores, which might write there for all the compiler knows
+                if (kSums && unit.index == 0) {
+                    const float* const from = V.state_of(seq.from, head) + at;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) first[e] = from[e * D];
+                }
+                tc::tmem_ld16(state_at + b, r);
                 tc::tmem_ld_wait();
                 if (row < D) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        float x = __uint_as_float(r[e]);
-                        if (kSums && unit.index == 0) x = fmaf(w, first[(col + e) * D + dim], x);
-                        to[(col + e) * D + dim] = x;
-                    }
+                    for (int e = 0; e < 16; ++e) to[at + e * D] = kSums && unit.index == 0 ? fmaf(w, first[e], __uint_as_float(r[e])) : __uint_as_float(r[e]);
                 }
                 __syncwarp();
             }
@@ -524,12 +573,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
         // ---- score warps: rows 0 .. 63 of the scores, 32 columns a warp
         const int quad = warp & 3, side = (warp - kLastWarps) >> 2, row = 32 * quad + lane, j0 = 32 * side;
         for (int c = 0; c < chunks; ++c) {
-            if (!wait2(sm.scores, c)) break;
+            if (!wait3(sm.rows_done, c)) break;
             tc::fence_after_sync();
             uint32_t s[32], p[16];
             float most = 0.0f;
             if (side <= quad) {  // a block with something on or below the diagonal
-                tc::tmem_ld32(tmem + (static_cast<uint32_t>(32 * quad) << 16) + kScoreCol + j0, s);
+                tc::tmem_ld32(tmem + (static_cast<uint32_t>(32 * quad) << 16) + kScoreCol + (c & 1) * kC + j0, s);
                 const int x0 = kC - 1 - row + j0, below = row - j0;  // columns 0 .. below are on or below the diagonal
                 const float2* const fade = reinterpret_cast<const float2*>(sm.fade[x0 & 1] + (x0 & ~1));
                 tc::tmem_ld_wait();
@@ -579,7 +628,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
         for (int c = 0; c < chunks; ++c) {
             const int64_t t = begin + c * kC;
             const int valid = min(kC, end - static_cast<int>(t));
-            if (!wait3(sm.done, c)) break;
+            if (!wait3(sm.done, c) || !wait3(sm.rows_done, c + 2)) break;
             if (!kBf16 && (!wait3(sm.state_ready, c) || !wait2(sm.p_ready, c))) break;  // sm.up, sm.inside of all rows
             if (c > 1 && !wait2(sm.out_free, c - 2)) break;
             tc::fence_after_sync();
@@ -588,7 +637,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
             for (int b = 0; b < kBlocks; ++b) {
                 const int i0 = first + kTokens * b;
                 uint32_t r[kTokens], s[kTokens];
-                tc::tmem_ld16(tmem + lanes + kInsideCol + (c & 1) * kC + i0, r);
+                tc::tmem_ld16(tmem + lanes + kInsideCol + i0, r);
                 tc::tmem_ld16(tmem + lanes + kBeforeCol + (c & 1) * kC + i0, s);
                 tc::tmem_ld_wait();
                 F2 zeros(0.0f, 0.0f);
@@ -635,7 +684,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
     if (failed && lane == 0 && V.error_word != nullptr) atomicOr(V.error_word, KVB_ERR_WAIT_TIMEOUT);
     tc::fence_before_sync();
     __syncthreads();
-    if (warp == kMmaWarp) {
+    if (warp == kStateMmaWarp) {
         tc::fence_after_sync();
         tc::tmem_dealloc(tmem, kTmemCols);
     }
@@ -649,7 +698,7 @@ template <int D, bool kBf16> int launch_chunks(const ChunkCall& P, int units, cu
         const cudaError_t e = cudaFuncSetAttribute(chunk_kernel<D, kBf16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         return e != cudaSuccess ? e : cudaFuncSetAttribute(chunk_kernel<D, kBf16, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     }));
-    const dim3 grid(units, P.V.v_heads);
+    const dim3 grid(P.V.v_heads, units);  // units that are none come last
     if (P.V.tokens > P.segment) KVB_CUDA_OK(launch_early(chunk_kernel<D, kBf16, true>, grid, dim3(kChunkThreads), smem, stream, P));
     KVB_CUDA_OK(launch_early(chunk_kernel<D, kBf16, false>, grid, dim3(kChunkThreads), smem, stream, P));
     return KVB_OK;
