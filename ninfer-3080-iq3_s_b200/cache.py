@@ -25,19 +25,25 @@ def _stream():
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
-def row_stride(x: torch.Tensor, heads: int, head_dim: int, dtype: torch.dtype, tokens: int | None = None) -> int:
+# Checks of the calls whose rows may be parts of wider ones.  A step makes them in every layer: what is right is seen in a few comparisons.
+def row_stride(x: torch.Tensor, heads: int, head_dim: int, dtype: torch.dtype, tokens: int) -> int:
     """Elements from token to token of rows [tokens, heads, head_dim] whose heads are packed; anything else is refused."""
-    if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != head_dim or x.dtype != dtype or (tokens is not None and x.shape[0] != tokens):
-        raise ValueError(f"rows [{'tokens' if tokens is None else tokens}, {heads}, {head_dim}] of {dtype}: got {tuple(x.shape)} of {x.dtype}")
-    at = x.stride()
-    if at[2] != 1 or (heads > 1 and at[1] != head_dim):
+    if x.shape == (tokens, heads, head_dim) and x.dtype is dtype:
+        at = x.stride()
+        if at[2] == 1 and (at[1] == head_dim or heads == 1):
+            return at[0]
         raise ValueError(f"the heads of a token lie packed: got strides {at}")
-    return at[0]
+    raise ValueError(f"rows [{tokens}, {heads}, {head_dim}] of {dtype}: got {tuple(x.shape)} of {x.dtype}")
 
 
-def check_positions(positions: torch.Tensor, tokens: int) -> None:
-    if positions.dtype != torch.int32 or positions.shape != (tokens,) or not positions.is_contiguous():
-        raise ValueError(f"positions: int32 [{tokens}], got {tuple(positions.shape)} of {positions.dtype}")
+def check_indices(x: torch.Tensor, n: int, name: str) -> int:
+    """The address of `n` packed int32 values."""
+    if x.shape == (n,) and x.dtype is _INT32 and (n < 2 or x.stride() == _PACKED):
+        return x.data_ptr()
+    raise ValueError(f"{name}: packed int32 [{n}], got {tuple(x.shape)} of {x.dtype}, strides {x.stride()}")
+
+
+_INT32, _PACKED = torch.int32, (1,)
 
 
 # Workspace sizes are functions of the shape (and of the device's SM count): a step asks for the same one in every layer.
@@ -78,6 +84,7 @@ class KvarnLayer:
             kv_heads=kv_heads, q_heads=q_heads, head_dim=head_dim,
             dtype=capi.DTYPE_BF16 if dtype == torch.bfloat16 else capi.DTYPE_F16, sinkhorn_iters=sinkhorn_iters,
             error_word=self.error_word.data_ptr())
+        self.ref = C.byref(self.c)
         self._ws = None
         self._pws = None
 
@@ -93,27 +100,28 @@ class KvarnLayer:
     def rope_append(self, rope, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, q: torch.Tensor | None = None, q_out: torch.Tensor | None = None):
         """k, v: [tokens, kv_heads, head_dim], q: [tokens, q_heads, head_dim], rows packed or parts of wider ones; `rope`: a rope.Rope.
         Returns the turned queries (None without q)."""
-        tokens, (kv, qh, d) = int(k.shape[0]), (self.kv_heads, self.q_heads, self.head_dim)
-        ks, vs = row_stride(k, kv, d, self.dtype, tokens), row_stride(v, kv, d, self.dtype, tokens)
-        check_positions(positions, tokens)
+        tokens, kv, qh, d, dtype = k.shape[0], self.kv_heads, self.q_heads, self.head_dim, self.dtype
+        ks, vs = row_stride(k, kv, d, dtype, tokens), row_stride(v, kv, d, dtype, tokens)
+        at = check_indices(positions, tokens, "positions")
         qs = os = 0
         if q is not None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
-            qs, os = row_stride(q, qh, d, self.dtype, tokens), row_stride(q_out, qh, d, self.dtype, tokens)
-        capi.check(capi.load().kvb_rope_append(C.byref(self.c), C.byref(rope.c), _ptr(q), qs, _ptr(q_out), os, _ptr(k), ks, _ptr(v), vs, _ptr(positions),
-                                               tokens, _stream()))
+            qs = row_stride(q, qh, d, dtype, tokens)
+            q_out = torch.empty_like(q) if q_out is None else q_out
+            os = row_stride(q_out, qh, d, dtype, tokens)
+        capi.check(capi.load().kvb_rope_append(self.ref, rope.ref, _ptr(q), qs, _ptr(q_out), os, k.data_ptr(), ks, v.data_ptr(), vs, at, tokens, _stream()))
         return q_out
 
     # ---- rows back as keys and values (the reference: its bf16 mirror, kvarn128_window*)
     def read_rows(self, begin: int, tokens: int, pos: torch.Tensor, out_k: torch.Tensor | None = None, out_v: torch.Tensor | None = None):
         """Rows [begin, begin + tokens) as [tokens, kv_heads, head_dim]; pos: int32 [1] on the device, the newest token's position."""
-        check_positions(pos, 1)
+        at = check_indices(pos, 1, "pos")
         shape = (tokens, self.kv_heads, self.head_dim)
-        out_k, out_v = (torch.empty(shape, dtype=self.dtype, device=self.device) if x is None else x for x in (out_k, out_v))
+        out_k = torch.empty(shape, dtype=self.dtype, device=self.device) if out_k is None else out_k
+        out_v = torch.empty_like(out_k) if out_v is None else out_v
         for x in (out_k, out_v):
-            if x.shape != shape or x.dtype != self.dtype or not x.is_contiguous():
+            if x.shape != shape or x.dtype is not self.dtype or not x.is_contiguous():
                 raise ValueError(f"outputs: packed rows {list(shape)} of {self.dtype}")
-        capi.check(capi.load().kvb_read_rows(C.byref(self.c), begin, tokens, _ptr(pos), _ptr(out_k), _ptr(out_v), _stream()))
+        capi.check(capi.load().kvb_read_rows(self.ref, begin, tokens, at, out_k.data_ptr(), out_v.data_ptr(), _stream()))
         return out_k, out_v
 
     # ---- kvarn128_decode_tile

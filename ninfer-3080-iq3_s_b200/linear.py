@@ -7,18 +7,12 @@ import functools
 import torch
 
 from . import capi
-from .cache import _ptr, _stream, row_stride
+from .cache import _stream, check_indices, row_stride
 
 
 @functools.lru_cache(maxsize=256)
 def _workspace_bytes(device, tokens, batch, v_heads, head_dim):
     return capi.load().kvb_linear_workspace_bytes(tokens, batch, v_heads, head_dim)
-
-
-def _check_indices(n, **indices):
-    for name, x in indices.items():
-        if x.dtype != torch.int32 or x.shape != (n,) or not x.is_contiguous():
-            raise ValueError(f"{name}: int32 [{n}], got {tuple(x.shape)} of {x.dtype}")
 
 
 class LinearAttention:
@@ -36,27 +30,27 @@ class LinearAttention:
         self.c = capi.kvb_linear(state=self.state.data_ptr(), log_decay=self.log_decay.data_ptr(), slots=slots, qk_heads=qk_heads, v_heads=v_heads,
                                  head_dim=head_dim, dtype=capi.DTYPE_BF16 if dtype == torch.bfloat16 else capi.DTYPE_F16,
                                  error_word=self.error_word.data_ptr())
+        self.ref = C.byref(self.c)
         self._ws = None
 
     def _device_key(self) -> int:
         return torch._C._cuda_getDevice() if self.device.type == "cuda" else -1
 
-    def _rows(self, q, k, v, out):
-        tokens = int(q.shape[0])
-        strides = [row_stride(x, h, self.head_dim, self.dtype, tokens) for x, h in ((q, self.qk_heads), (k, self.qk_heads), (v, self.v_heads))]
+    def _out(self, tokens, v, out):
         if out is None:
-            out = torch.empty((tokens, self.v_heads, self.head_dim), dtype=self.dtype, device=q.device)
-        elif out.shape != (tokens, self.v_heads, self.head_dim) or out.dtype != self.dtype or not out.is_contiguous():
+            return torch.empty((tokens, self.v_heads, self.head_dim), dtype=self.dtype, device=v.device) if not v.is_contiguous() else torch.empty_like(v)
+        if out.shape != (tokens, self.v_heads, self.head_dim) or out.dtype is not self.dtype or not out.is_contiguous():
             raise ValueError(f"out: packed rows [{tokens}, {self.v_heads}, {self.head_dim}] of {self.dtype}")
-        return tokens, strides, out
+        return out
 
     def decode(self, q, k, v, scale: float, reads: torch.Tensor, writes: torch.Tensor, out=None) -> torch.Tensor:
         """One token of each sequence: q, k [batch, qk_heads, head_dim], v [batch, v_heads, head_dim]; reads, writes: int32 [batch] on the device, the
         slots a sequence's state is read from and written to (the same one for a step in place)."""
-        batch, (qs, ks, vs), out = self._rows(q, k, v, out)
-        _check_indices(batch, reads=reads, writes=writes)
-        capi.check(capi.load().kvb_linear_decode(C.byref(self.c), _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, batch, _ptr(reads), _ptr(writes), scale,
-                                                 _ptr(out), _stream()))
+        batch, qk, d, dtype = q.shape[0], self.qk_heads, self.head_dim, self.dtype
+        qs, ks, vs = row_stride(q, qk, d, dtype, batch), row_stride(k, qk, d, dtype, batch), row_stride(v, self.v_heads, d, dtype, batch)
+        out = self._out(batch, v, out)
+        capi.check(capi.load().kvb_linear_decode(self.ref, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, batch, check_indices(reads, batch, "reads"),
+                                                 check_indices(writes, batch, "writes"), scale, out.data_ptr(), _stream()))
         return out
 
     def workspace(self, tokens: int, batch: int) -> torch.Tensor:
@@ -69,12 +63,12 @@ class LinearAttention:
 
     def chunk(self, q, k, v, offsets: torch.Tensor, scale: float, reads: torch.Tensor, writes: torch.Tensor, out=None) -> torch.Tensor:
         """Several tokens of each sequence, packed: rows offsets[b] .. offsets[b + 1] - 1 are sequence b's; offsets: int32 [batch + 1] on the device."""
-        tokens, (qs, ks, vs), out = self._rows(q, k, v, out)
-        batch = int(reads.shape[0])
-        _check_indices(batch, reads=reads, writes=writes)
-        _check_indices(batch + 1, offsets=offsets)
-        capi.check(capi.load().kvb_linear_chunk(C.byref(self.c), _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(offsets), batch, tokens, _ptr(reads),
-                                                _ptr(writes), scale, _ptr(self.workspace(tokens, batch)), _ptr(out), _stream()))
+        tokens, qk, d, dtype, batch = q.shape[0], self.qk_heads, self.head_dim, self.dtype, reads.shape[0]
+        qs, ks, vs = row_stride(q, qk, d, dtype, tokens), row_stride(k, qk, d, dtype, tokens), row_stride(v, self.v_heads, d, dtype, tokens)
+        out = self._out(tokens, v, out)
+        capi.check(capi.load().kvb_linear_chunk(self.ref, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, check_indices(offsets, batch + 1, "offsets"),
+                                                batch, tokens, check_indices(reads, batch, "reads"), check_indices(writes, batch, "writes"), scale,
+                                                self.workspace(tokens, batch).data_ptr(), out.data_ptr(), _stream()))
         return out
 
     def errors(self) -> int:

@@ -7,9 +7,10 @@ import ctypes as C
 import torch
 
 from . import capi
-from .cache import _ptr, _stream, check_positions, row_stride
+from .cache import _stream, check_indices, row_stride
 
 _SCALINGS = {"none": capi.ROPE_PLAIN, "linear": capi.ROPE_LINEAR, "ntk": capi.ROPE_NTK, "yarn": capi.ROPE_YARN}
+_DTYPES = {torch.float16: capi.DTYPE_F16, torch.bfloat16: capi.DTYPE_BF16}
 
 
 class Rope:
@@ -25,15 +26,17 @@ class Rope:
         self.rotary_dim, self.factor, self.interleaved = rotary_dim, attention.value, interleaved
         self.inv_freq = torch.tensor(list(host), dtype=torch.float64).to(device)
         self.c = capi.kvb_rope(inv_freq=self.inv_freq.data_ptr(), factor=self.factor, rotary_dim=rotary_dim, interleaved=int(interleaved))
+        self.ref = C.byref(self.c)
 
     def rows(self, x: torch.Tensor, positions: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """x: [tokens, heads, head_dim] (fp16 or bf16), packed or part of wider rows; positions: int32 [tokens] on the device.  `out` may be x."""
-        if x.dtype not in (torch.float16, torch.bfloat16) or x.dim() != 3:
+        dtype = _DTYPES.get(x.dtype)
+        if dtype is None or x.dim() != 3:
             raise ValueError(f"x: rows [tokens, heads, head_dim] of float16 or bfloat16, got {tuple(x.shape)} of {x.dtype}")
         tokens, heads, dim = x.shape
-        check_positions(positions, tokens)
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
-        capi.check(capi.load().kvb_rope_rows(C.byref(self.c), _ptr(x), row_stride(x, heads, dim, x.dtype), _ptr(out),
-                                             row_stride(out, heads, dim, x.dtype, tokens), _ptr(positions), tokens, heads, dim,
-                                             capi.DTYPE_BF16 if x.dtype == torch.bfloat16 else capi.DTYPE_F16, _stream()))
+        at = check_indices(positions, tokens, "positions")
+        stride = row_stride(x, heads, dim, x.dtype, tokens)
+        out = torch.empty_like(x) if out is None else out
+        capi.check(capi.load().kvb_rope_rows(self.ref, x.data_ptr(), stride, out.data_ptr(), row_stride(out, heads, dim, x.dtype, tokens), at, tokens, heads,
+                                             dim, dtype, _stream()))
         return out

@@ -165,9 +165,13 @@ def test_python_refuses_rows_that_are_not_rows():
     row_stride = import_module("kvarn_b200.cache").row_stride
     x = torch.zeros((5, 7, 128), dtype=torch.float16)
     assert row_stride(x, 7, 128, torch.float16, 5) == 7 * 128
-    assert row_stride(x[:, :3], 3, 128, torch.float16) == 7 * 128
-    for bad in ((x.bfloat16(), 7, 128), (x, 6, 128), (x, 7, 64), (x[0], 7, 128), (x.transpose(0, 1), 5, 128), (x[..., ::2], 7, 64), (x[:, ::2], 4, 128)):
+    assert row_stride(x[:, :3], 3, 128, torch.float16, 5) == 7 * 128
+    for bad in ((x.bfloat16(), 7, 128), (x, 6, 128), (x, 7, 64), (x[0], 7, 128), (x.transpose(0, 1), 5, 128), (x[..., ::2], 7, 64), (x[:, ::2], 4, 128), (x[:4], 7, 128)):
         with pytest.raises(ValueError):
-            row_stride(*bad, torch.float16)
-    with pytest.raises(ValueError):
-        row_stride(x, 7, 128, torch.float16, 4)
+            row_stride(*bad, torch.float16, 5)
+    check_indices = import_module("kvarn_b200.cache").check_indices
+    at = torch.arange(8, dtype=torch.int32)
+    assert check_indices(at, 8, "x") == at.data_ptr() and check_indices(at[3:4], 1, "x") == at[3:].data_ptr() and check_indices(at[:0], 0, "x") is not None
+    for bad in ((at, 7), (at.long(), 8), (at[::2], 4), (at.view(2, 4), 8)):
+        with pytest.raises(ValueError):
+            check_indices(*bad, "x")
