@@ -302,37 +302,83 @@ __device__ void quantize_slice(AppendSmem& sm, float (&x)[kPer]) {
     __syncthreads();
 }
 
+__host__ __device__ constexpr int rope_row_floats(int rotary) { return (rotary + 31) / 32 * 32 + 4; }  // whole groups of place()'s order, and a word for the banks
+__host__ __device__ constexpr int rope_bytes(int rotary, int rows) { return rows * rope_row_floats(rotary) * static_cast<int>(sizeof(float)) + (rotary + 2) / 4 * 2 * static_cast<int>(sizeof(uint64_t)); }
+
 // What happens to a row between global memory and its Walsh-Hadamard rotation: nothing, or the turn of its position.
 struct NoTurn {
     static constexpr bool kTurns = false;
     __device__ __forceinline__ void ready() const {}
 };
-// The angles of a tile's new rows meet in shared memory, [row][pair], each computed once for the CTA's head; that runs while the rows are
-// under way from global memory.  Rows of fp32 go on to the Walsh-Hadamard rotation: nothing is rounded in between.
-struct RopeTurn {
+// The turning dims of a tile's new rows, turned by the whole CTA, in shared memory as fp32: nothing is rounded before the Walsh-Hadamard rotation reads
+// them there.  That runs while the other dims are under way from global memory.  A thread turns 8 pairs of a row (16 bytes of either half), or one pair
+// where the rows are few or not made for that.  Angles are products of a pair's turns per position, as 64-bit fractions, and the position.
+// Measured on B200 against a table of the angles, each row's lanes turning their own dims (graph replay, without queries): 777 tokens of 128 dims
+// 10.9 -> 10.1 us, 1,024 of 256 dims 13.3 -> 11.3; the plain append 6.8 and 9.1.
+template <bool kBf16> struct RopeTurn {
     static constexpr bool kTurns = true;
     RopeView rope;
-    float2* table;
-    int stride;  // entries from row to row: an odd number of 16-byte words more than the pairs, so that rows fall on different banks
+    float* turned;    // [row][turning dim], in the order of place()
+    uint64_t* steps;  // of the pairs
+    const uint16_t* src;
+    int64_t row_stride;
     int first, rows;  // position of the tile's first new row, and their number
+    bool wide;
+
+    // 16-byte words of a row: the lanes of a row read words 8 apart, which lie in different banks
+    __device__ __forceinline__ int place(int row, int d) const {
+        const int word = d >> 2;
+        return row * rope_row_floats(rope.rotary) + ((word ^ ((word >> 3) & 7)) << 2) + (d & 3);
+    }
     __device__ __forceinline__ void ready() const {
         const int pairs = rope.rotary / 2;
-        for (int i = threadIdx.x; i < rows * pairs; i += kThreads) {
-            const int r = i / pairs, p = i - r * pairs;
-            table[r * stride + p] = rope_turn(rope.inv_freq[p], first + r, rope.factor);
+        if (static_cast<int>(threadIdx.x) < pairs) steps[threadIdx.x] = rope_step(rope.inv_freq[threadIdx.x]);
+        __syncthreads();
+        auto angle = [&](int pair, int row) { return rope_turn_of(steps[pair] * static_cast<uint64_t>(static_cast<int64_t>(first + row)), rope.factor); };
+        if (wide && rows * pairs > 2 * kThreads) {
+            const int units = rope.interleaved ? rope.rotary / 8 : rope.rotary / 16;
+            for (int i = threadIdx.x; i < rows * units; i += kThreads) {
+                const int row = i / units, unit = i - row * units;
+                const uint16_t* const from = src + row * row_stride + 8 * unit;
+                float x[8], y[8];
+                unpack8_16<kBf16>(*reinterpret_cast<const uint4*>(from), x);
+                if (rope.interleaved) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 t = angle(4 * unit + e, row);
+                        y[2 * e] = turn_first(x[2 * e], x[2 * e + 1], t);
+                        y[2 * e + 1] = turn_second(x[2 * e + 1], x[2 * e], t);
+                    }
+                    *reinterpret_cast<float4*>(&turned[place(row, 8 * unit)]) = make_float4(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<float4*>(&turned[place(row, 8 * unit + 4)]) = make_float4(y[4], y[5], y[6], y[7]);
+                } else {
+                    unpack8_16<kBf16>(*reinterpret_cast<const uint4*>(from + pairs), y);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float2 t = angle(8 * unit + e, row);
+                        const float a = x[e], b = y[e];
+                        x[e] = turn_first(a, b, t);
+                        y[e] = turn_second(b, a, t);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; e += 4) {
+                        *reinterpret_cast<float4*>(&turned[place(row, 8 * unit + e)]) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+                        *reinterpret_cast<float4*>(&turned[place(row, pairs + 8 * unit + e)]) = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+                    }
+                }
+            }
+        } else {
+            for (int i = threadIdx.x; i < rows * pairs; i += kThreads) {
+                const int row = i / pairs, pair = i - row * pairs, a = rope.interleaved ? 2 * pair : pair, b = rope.interleaved ? a + 1 : pair + pairs;
+                const float x = in_to_f32<kBf16>(src[row * row_stride + a]), y = in_to_f32<kBf16>(src[row * row_stride + b]);
+                const float2 t = angle(pair, row);
+                turned[place(row, a)] = turn_first(x, y, t);
+                turned[place(row, b)] = turn_second(y, x, t);
+            }
         }
         __syncthreads();
     }
-    // dim d's other half, its pair, and whether d is the pair's first
-    __device__ __forceinline__ int peer(int d) const { return rope.interleaved ? d ^ 1 : d < rope.rotary / 2 ? d + rope.rotary / 2 : d - rope.rotary / 2; }
-    __device__ __forceinline__ int pair(int d) const { return rope.interleaved ? d >> 1 : d < rope.rotary / 2 ? d : d - rope.rotary / 2; }
-    __device__ __forceinline__ bool is_first(int d) const { return rope.interleaved ? (d & 1) == 0 : d < rope.rotary / 2; }
-    __device__ __forceinline__ float turned(int row, int d, float x, float other) const {
-        const float2 t = table[row * stride + pair(d)];
-        return is_first(d) ? turn_first(x, other, t) : turn_second(x, other, t);
-    }
 };
-__host__ __device__ constexpr int rope_table_stride(int rotary) { return (rotary / 2 + 1) / 2 * 2 + 2; }
 
 // The new rows begin .. end - 1 of tile `base`, rotated (stages, order and roundings of hadamard_warp).  A lane holds 32 neighbouring
 // dims of a row: D / 32 lanes a row, 1024 / D rows a warp at a time; the strides up to 16 stay inside a lane, in pairs of dims, those of
@@ -351,19 +397,10 @@ __device__ __forceinline__ void rotate_rows(const uint16_t* __restrict__ src, in
         const int tt = begin + warp + kWarpsPerCta * (u * kAtOnce + lane / kLanes);
         const uint16_t* row = src + (tt - begin) * row_stride + 32 * block;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) raw[u][c] = tt >= end ? make_uint4(0u, 0u, 0u, 0u) : reinterpret_cast<const uint4*>(row)[c];
-    }
-    uint4 other[Turn::kTurns ? kPasses : 1][4];  // the other halves of the same pairs
-    if constexpr (Turn::kTurns) {
-#pragma unroll
-        for (int u = 0; u < kPasses; ++u) {
-            const int tt = begin + warp + kWarpsPerCta * (u * kAtOnce + lane / kLanes);
-            const uint16_t* row = src + (tt - begin) * row_stride;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int d = 32 * block + 8 * c;
-                other[u][c] = tt < end && d < turn.rope.rotary && !turn.rope.interleaved ? *reinterpret_cast<const uint4*>(row + turn.peer(d)) : make_uint4(0u, 0u, 0u, 0u);
-            }
+        for (int c = 0; c < 4; ++c) {
+            bool there = tt < end;
+            if constexpr (Turn::kTurns) there = there && 32 * block + 8 * c >= turn.rope.rotary;
+            raw[u][c] = there ? reinterpret_cast<const uint4*>(row)[c] : make_uint4(0u, 0u, 0u, 0u);
         }
     }
     turn.ready();
@@ -379,28 +416,8 @@ __device__ __forceinline__ void rotate_rows(const uint16_t* __restrict__ src, in
             if constexpr (Turn::kTurns) {
                 const int d = 32 * block + 8 * c;
                 if (d < turn.rope.rotary && tt < end) {
-                    const float4* t = reinterpret_cast<const float4*>(turn.table + (tt - begin) * turn.stride + turn.pair(d));
-                    if (turn.rope.interleaved) {
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float4 a = t[e];
-                            const float y0 = y[4 * e], y1 = y[4 * e + 1], y2 = y[4 * e + 2], y3 = y[4 * e + 3];
-                            y[4 * e] = turn_first(y0, y1, make_float2(a.x, a.y));
-                            y[4 * e + 1] = turn_second(y1, y0, make_float2(a.x, a.y));
-                            y[4 * e + 2] = turn_first(y2, y3, make_float2(a.z, a.w));
-                            y[4 * e + 3] = turn_second(y3, y2, make_float2(a.z, a.w));
-                        }
-                    } else {
-                        float z[8];
-                        unpack8_16<kBf16>(other[u][c], z);
-                        const float sign = turn.is_first(d) ? -1.0f : 1.0f;  // exact, so both halves are one formula
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float4 a = t[e];
-                            y[2 * e] = turn_second(y[2 * e], z[2 * e], make_float2(a.x, __fmul_rn(a.y, sign)));
-                            y[2 * e + 1] = turn_second(y[2 * e + 1], z[2 * e + 1], make_float2(a.z, __fmul_rn(a.w, sign)));
-                        }
-                    }
+                    const float4 lo = *reinterpret_cast<const float4*>(&turn.turned[turn.place(tt - begin, d)]), hi = *reinterpret_cast<const float4*>(&turn.turned[turn.place(tt - begin, d + 4)]);
+                    y[0] = lo.x, y[1] = lo.y, y[2] = lo.z, y[3] = lo.w, y[4] = hi.x, y[5] = hi.y, y[6] = hi.z, y[7] = hi.w;
                 }
             }
 #pragma unroll
@@ -457,21 +474,6 @@ __device__ __forceinline__ void rotate_rows_singly(const uint16_t* __restrict__ 
             for (int r = 0; r < D / 32; ++r) raw[u][r] = row[lane + 32 * r];
         }
     }
-    // the other halves of the pairs: asked for beside the rows where there are few of them, else as they are needed, out of the L1
-    constexpr bool kAhead = Turn::kTurns && kBatch <= 3;
-    uint16_t other[kAhead ? kBatch : 1][D / 32];
-    if constexpr (kAhead) {
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-            const int tt = begin + warp + u * kWarpsPerCta;
-            if (tt < end) {
-                const uint16_t* row = src + (tt - begin) * row_stride;
-#pragma unroll
-                for (int r = 0; r < D / 32; ++r)
-                    if (lane + 32 * r < turn.rope.rotary) other[u][r] = row[turn.peer(lane + 32 * r)];
-            }
-        }
-    }
     turn.ready();
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
@@ -483,10 +485,7 @@ __device__ __forceinline__ void rotate_rows_singly(const uint16_t* __restrict__ 
             val[r] = in_to_f32<kBf16>(raw[u][r]);
             if constexpr (Turn::kTurns) {
                 const int d = lane + 32 * r;
-                if (d < turn.rope.rotary) {
-                    const uint16_t z = kAhead ? other[kAhead ? u : 0][r] : src[(tt - begin) * row_stride + turn.peer(d)];
-                    val[r] = turn.turned(tt - begin, d, val[r], in_to_f32<kBf16>(z));
-                }
+                if (d < turn.rope.rotary) val[r] = turn.turned[turn.place(tt - begin, d)];
             }
         }
         hadamard_warp<D>(val, lane);
@@ -519,7 +518,7 @@ struct AppendRope {
     RopeView rope;
     RopeRows q;    // q.x null: no queries
     int64_t k_stride, v_stride;
-    int tiles, table_stride;
+    int tiles;
     bool wide_k, wide_v, wide_q;
 };
 struct NoRope {};
@@ -589,7 +588,8 @@ __global__ void __launch_bounds__(kThreads, 1) append_kernel(LayerView L, const 
         };
         if constexpr (kRope) {
             if (!which) {
-                by_size(RopeTurn{R.rope, reinterpret_cast<float2*>(smem_raw + sizeof(AppendSmem)), R.table_stride, a.base + a.begin, a.end - a.begin});
+                uint64_t* const steps = reinterpret_cast<uint64_t*>(smem_raw + sizeof(AppendSmem));
+                by_size(RopeTurn<kBf16>{R.rope, reinterpret_cast<float*>(steps + (R.rope.rotary + 2) / 4 * 2), steps, rows, row_stride, a.base + a.begin, a.end - a.begin, wide});
                 return;
             }
         }
@@ -704,20 +704,21 @@ int launch_append(const LayerView& V, const void* k, const void* v, const int32_
 
 template <int D, bool kBf16>
 int launch_rope_append(const LayerView& V, AppendRope R, const void* k, const void* v, const int32_t* positions, int tokens, cudaStream_t stream) {
-    static_assert(sizeof(AppendSmem) % 16 == 0 && sizeof(AppendSmem) + kTile * sizeof(float2) * rope_table_stride(D) <= 227 * 1024, "shared memory");
+    constexpr int most = static_cast<int>(sizeof(AppendSmem)) + rope_bytes(D, kTile);
+    static_assert(sizeof(AppendSmem) % 16 == 0 && most <= 227 * 1024, "shared memory");
     static OncePerDevice opted;  // per template instance
-    KVB_CUDA_OK(allow_smem(opted, append_kernel<D, kBf16, true>, static_cast<int>(sizeof(AppendSmem) + kTile * sizeof(float2) * rope_table_stride(D))));
+    KVB_CUDA_OK(allow_smem(opted, append_kernel<D, kBf16, true>, most));
     R.tiles = tokens / kTile + 2;
-    R.table_stride = rope_table_stride(R.rope.rotary);
-    const int smem = static_cast<int>(sizeof(AppendSmem) + (tokens < kTile ? tokens : kTile) * sizeof(float2) * R.table_stride);
-    // the queries' items: a CTA's threads once over, in whole columns of the grid, on no more CTAs than the device has SMs
+    const int smem = static_cast<int>(sizeof(AppendSmem)) + rope_bytes(R.rope.rotary, tokens < kTile ? tokens : kTile);
+    // The queries are the same launch's where all of its CTAs are resident at once (one an SM), in whole columns of the grid; else a launch beside it,
+    // whose smaller CTAs take the SMs that the append leaves.  Measured on B200, 1,024 tokens of 4 and 24 heads of 256 dims: 20.8 us as one launch, 19.6 as two.
     const int column = V.kv_heads * 2 * Geo<D>::S;
-    int64_t ctas = R.q.x == nullptr ? 0 : (R.q.items + kThreads - 1) / kThreads;
-    if (ctas > device_sm_count()) ctas = device_sm_count();
-    const dim3 grid(R.tiles + static_cast<unsigned>((ctas + column - 1) / column), V.kv_heads, 2 * Geo<D>::S);
+    const int64_t ctas = R.q.x == nullptr ? 0 : (R.q.items + kThreads - 1) / kThreads, columns = (ctas + column - 1) / column;
+    const bool beside = (R.tiles + columns) * column > device_sm_count();
+    const dim3 grid(R.tiles + (beside ? 0 : static_cast<unsigned>(columns)), V.kv_heads, 2 * Geo<D>::S);
     KVB_CUDA_OK(launch_early(append_kernel<D, kBf16, true>, grid, dim3(kThreads), smem, stream, V, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
                              positions, tokens, R));
-    return KVB_OK;
+    return beside && ctas > 0 ? launch_rope(R.q, kBf16, R.wide_q, true, stream) : KVB_OK;
 }
 
 }  // namespace

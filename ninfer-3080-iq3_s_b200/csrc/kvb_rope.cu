@@ -41,16 +41,24 @@ RopeRows rope_rows_of(const kvb_rope& rope, const void* x, void* out, const int3
 
 namespace {
 
-constexpr int kRopeThreads = 128;
-
-template <bool kBf16, bool kWide> __global__ void __launch_bounds__(kRopeThreads) rope_kernel(RopeRows P) {
-    grid_dependency_wait();
+template <bool kBf16, bool kWide> __global__ void __launch_bounds__(kRopeThreads) rope_kernel(RopeRows P, bool beside) {
+    if (!beside) grid_dependency_wait();
     launch_dependents();
     const int64_t item = static_cast<int64_t>(blockIdx.x) * kRopeThreads + threadIdx.x;
     if (item < P.items) rope_item<kBf16, kWide>(P, item);
+    if (beside) grid_dependency_wait();  // nobody leaves before the append is over: what waits for this grid finds both done
 }
 
 }  // namespace
+
+int launch_rope(const RopeRows& P, bool bf16, bool wide, bool beside, cudaStream_t stream) {
+    const int64_t blocks = (P.items + kRopeThreads - 1) / kRopeThreads;
+    if (blocks > INT32_MAX) return fail(KVB_ERANGE, "rotary positions: too many rows for one call");
+    auto* kernel = wide ? (bf16 ? rope_kernel<true, true> : rope_kernel<false, true>) : (bf16 ? rope_kernel<true, false> : rope_kernel<false, false>);
+    KVB_CUDA_OK(launch_early(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kRopeThreads), 0, stream, P, beside));
+    return KVB_OK;
+}
+
 }  // namespace kvb
 
 extern "C" int kvb_rope_frequencies(int rotary_dim, double base, int scaling, double factor, int original_len, double* inv_freq, float* attention_factor) {
@@ -104,10 +112,5 @@ extern "C" int kvb_rope_rows(const kvb_rope* rope, const void* x, int64_t x_stri
         return fail(KVB_EINVAL, "kvb_rope_rows: out shares memory with the positions or frequencies");
     const bool wide = rope_is_wide(*rope, head_dim, x, out, x_stride, out_stride);
     const RopeRows P = rope_rows_of(*rope, x, out, positions_dev, tokens, heads, head_dim, x_stride, out_stride, wide);
-    const int64_t blocks = (P.items + kRopeThreads - 1) / kRopeThreads;
-    if (blocks > INT32_MAX) return fail(KVB_ERANGE, "kvb_rope_rows: %d tokens are too many for one call", tokens);
-    const bool bf = dtype == KVB_DTYPE_BF16;
-    auto* kernel = wide ? (bf ? rope_kernel<true, true> : rope_kernel<false, true>) : (bf ? rope_kernel<true, false> : rope_kernel<false, false>);
-    KVB_CUDA_OK(launch_early(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kRopeThreads), 0, static_cast<cudaStream_t>(stream), P));
-    return KVB_OK;
+    return launch_rope(P, dtype == KVB_DTYPE_BF16, wide, false, static_cast<cudaStream_t>(stream));
 }

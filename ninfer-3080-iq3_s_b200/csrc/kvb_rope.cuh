@@ -26,6 +26,17 @@ __device__ __forceinline__ float2 rope_turn(double inv_freq, int position, float
     sincospif(2.0f * static_cast<float>(turns), &s, &c);
     return make_float2(__fmul_rn(c, factor), __fmul_rn(s, factor));
 }
+// The same for positions in a row: turns as 64-bit fractions of one, whose products and sums with whole numbers of positions are exact but for whole
+// turns, so that the next position costs an addition.  `step`: turns per position, rounded to 2^-55 of one.
+__device__ __forceinline__ uint64_t rope_step(double inv_freq) {
+    const double turns = __dmul_rn(inv_freq, 0.15915494309189533577);
+    return __double2ull_rz(__dmul_rn(turns - floor(turns), 18446744073709551616.0));
+}
+__device__ __forceinline__ float2 rope_turn_of(uint64_t phase, float factor) {
+    float s, c;
+    sincospif(static_cast<float>(static_cast<int32_t>((phase + 0x80000000u) >> 32)) * 0x1p-31f, &s, &c);
+    return make_float2(__fmul_rn(c, factor), __fmul_rn(s, factor));
+}
 __device__ __forceinline__ float turn_first(float x, float peer, float2 t) { return __fmaf_rn(x, t.x, -__fmul_rn(peer, t.y)); }
 __device__ __forceinline__ float turn_second(float x, float peer, float2 t) { return __fmaf_rn(x, t.x, __fmul_rn(peer, t.y)); }
 
@@ -58,6 +69,8 @@ template <bool kBf16> __device__ __forceinline__ uint4 pack8_16(const float (&f)
 
 // Heads of a thread whose loads are under way at once.
 constexpr int kRopeAtOnce = 4;
+
+constexpr int kRopeThreads = 128;
 
 template <bool kBf16, bool kWide> __device__ __forceinline__ void rope_item(const RopeRows& P, int64_t item) {
     const int unit = static_cast<int>(item % P.units);
@@ -144,6 +157,8 @@ template <bool kBf16, bool kWide> __device__ __forceinline__ void rope_item(cons
 
 // ---- host side ----------------------------------------------------------------------------------------------------------------
 int check_rope(const kvb_rope* rope, int head_dim, const char* who);
+// Turns rows, beside the append right before it in the stream where `beside` (kvb_step.hpp): nothing that it touches is the append's.
+int launch_rope(const RopeRows& P, bool bf16, bool wide, bool beside, cudaStream_t stream);
 // Whether rows, distances and the turning part allow 16-byte accesses.
 inline bool rope_is_wide(const kvb_rope& rope, int head_dim, const void* x, const void* out, int64_t x_stride, int64_t out_stride) {
     const int whole = rope.interleaved ? 8 : 16;
