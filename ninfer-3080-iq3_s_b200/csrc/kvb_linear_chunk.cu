@@ -42,7 +42,7 @@ constexpr int kStages = 3;
 constexpr int kStateWarps = 8, kRowWarps = 8;
 // the last eight: warps 0, 1, 4, 5 of them P (rows 0 .. 63 of tensor memory are a warp's by its number mod 4)
 constexpr int kLastWarps = kStateWarps + kRowWarps, kStateMmaWarp = kLastWarps + 2, kLoadWarp = kLastWarps + 3, kRowMmaWarp = kLastWarps + 6, kStoreWarp = kLastWarps + 7;
-constexpr int kStateThreads = kStateWarps * 32, kRowThreads = kRowWarps * 32, kScoreThreads = 128;
+constexpr int kStateThreads = kStateWarps * 32, kScoreWarps = 4;
 constexpr int kChunkThreads = (kLastWarps + 8) * 32;  // 24 warps: six to a scheduler, 80 registers a thread
 constexpr uint32_t kTmemCols = 512;
 
@@ -55,8 +55,8 @@ template <int D> struct LinearSmem {
     unsigned char second[2][kTileBytes];   // their second numbers, of two chunks
     unsigned char p[2][kC * kC * 2];       // P of two chunks
     uint32_t out[2][kTileBytes / 4];       // outputs of two chunks, [32 pairs of tokens][D]
-    float fade[2][2 * kC];                 // fade[s][x] = lambda^(63 - x - s), 0 behind lambda^0; the second copy for aligned pairs from odd x on
-    float before[kC];                      // scale lambda^(i + 1)
+    float fade[2][2 * kC + 16];            // fade[s][x] = lambda^(63 - x - s), 0 behind lambda^0; the second copy for aligned pairs from odd x on, 16 banks further
+    alignas(16) float before[kC];                      // scale lambda^(i + 1)
     float inside[2][kC];                   // scale times what P's row i was scaled down by (fp16)
     uint8_t up[3][128];                    // exponent field of what a row of the state was scaled down by (fp16)
     uint8_t most_state[2][128], most_p[2][2][kC];  // exponents of the largest magnitudes of a row, one a column half (fp16)
@@ -244,18 +244,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
             mbar_init(&sm.full[s], 1);
             mbar_init(&sm.done[s], 1);
             mbar_init(&sm.rows_done[s], 1);
-            mbar_init(&sm.state_ready[s], kStateThreads);
+            mbar_init(&sm.state_ready[s], kStateWarps);
         }
         for (int s = 0; s < 2; ++s) {
-            mbar_init(&sm.p_ready[s], kScoreThreads);
-            mbar_init(&sm.keys_ready[s], kStateThreads);
-            mbar_init(&sm.out_read[s], kRowThreads);
-            mbar_init(&sm.out_ready[s], kRowThreads);
+            mbar_init(&sm.p_ready[s], kScoreWarps);
+            mbar_init(&sm.keys_ready[s], kStateWarps);
+            mbar_init(&sm.out_read[s], kRowWarps);
+            mbar_init(&sm.out_ready[s], kRowWarps);
             mbar_init(&sm.out_free[s], 1);
         }
-        mbar_init(&sm.most_ready[0], kStateThreads);
-        mbar_init(&sm.most_ready[1], kScoreThreads);
-        mbar_init(&sm.loaded, kStateThreads + kRowThreads);
+        mbar_init(&sm.most_ready[0], kStateWarps);
+        mbar_init(&sm.most_ready[1], kScoreWarps);
+        mbar_init(&sm.loaded, kStateWarps + kRowWarps);
         mbar_init(&sm.drained[0], 1);
         mbar_init(&sm.drained[1], 1);
         mbar_fence_init();
@@ -274,6 +274,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
     auto wait = [&](uint64_t* bar, int phase) {
         if (!failed && !chunk_wait(bar, static_cast<uint32_t>(phase & 1), &sm.abort_flag)) failed = true;
         return !failed;
+    };
+    // one arrival a warp, when all its lanes are there (256 a barrier kept shared memory busy)
+    auto arrive = [&](uint64_t* bar) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
     };
     auto wait2 = [&](uint64_t (&bars)[2], int c) { return wait(&bars[c & 1], c >> 1); };
     auto wait3 = [&](uint64_t (&bars)[3], int c) { return wait(&bars[c % 3], c / 3); };
@@ -318,7 +323,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
         if (!kSums) {
             tc::tmem_st_wait();
             tc::fence_before_sync();
-            mbar_arrive(&sm.loaded);
+            arrive(&sm.loaded);
         }
     }
     if (warp == kLoadWarp) {
@@ -473,11 +478,23 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                 if (j >= valid) raw = make_uint4(0u, 0u, 0u, 0u);
                 const uint32_t in[4] = {raw.x, raw.y, raw.z, raw.w};
                 uint32_t a[4], b[4];
+                if constexpr (kBf16) {
+                    // the weight as two numbers, too: the first product rounded, what that left out (exact) and the second product
+                    const __nv_bfloat16 first = __float2bfloat16_rn(w);
+                    const __nv_bfloat162 w1 = __bfloat162bfloat162(first), w2 = __bfloat162bfloat162(__float2bfloat16_rn(w - __bfloat162float(first)));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const F2 x = mul2(pair_of<kBf16>(in[e]), F2(w, w));
-                    a[e] = pack_pair<kBf16>(x);
-                    b[e] = pack_pair<kBf16>(sub2(x, pair_of<kBf16>(a[e])));
+                    for (int e = 0; e < 4; ++e) {
+                        const __nv_bfloat162 k = *reinterpret_cast<const __nv_bfloat162*>(&in[e]), x = __hmul2(k, w1), y = __hfma2(k, w2, __hfma2(k, w1, __hneg2(x)));
+                        a[e] = *reinterpret_cast<const uint32_t*>(&x);
+                        b[e] = *reinterpret_cast<const uint32_t*>(&y);
+                    }
+                } else {  // small weights have too few bits in fp16
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const F2 x = mul2(pair_of<kBf16>(in[e]), F2(w, w));
+                        a[e] = pack_pair<kBf16>(x);
+                        b[e] = pack_pair<kBf16>(sub2(x, pair_of<kBf16>(a[e])));
+                    }
                 }
                 *reinterpret_cast<uint4*>(keys + 16 * u) = make_uint4(a[0], a[1], a[2], a[3]);
                 *reinterpret_cast<uint4*>(second + 16 * u) = make_uint4(b[0], b[1], b[2], b[3]);
@@ -487,7 +504,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                     if (((u >> 3) & (kC - 1)) >= valid) *reinterpret_cast<uint4*>(sm.stage[c % kStages].v + 16 * u) = make_uint4(0u, 0u, 0u, 0u);
             }
             fence_proxy_async();
-            mbar_arrive(&sm.keys_ready[c & 1]);
+            arrive(&sm.keys_ready[c & 1]);
         };
         if (kSums) {
             for (int c = 0; c < chunks && !failed; ++c) {
@@ -516,7 +533,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                     }
                     const int mine = static_cast<int>(__float_as_uint(most) >> 23);
                     sm.most_state[side][row] = static_cast<uint8_t>(mine);
-                    mbar_arrive(&sm.most_ready[0]);
+                    arrive(&sm.most_ready[0]);
                     if (!wait(&sm.most_ready[0], c)) break;
                     const int2 f = down_and_up(max(mine, static_cast<int>(sm.most_state[side ^ 1][row])));
                     down = of_field(f.x);
@@ -540,7 +557,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                 }
                 tc::tmem_st_wait();
                 tc::fence_before_sync();
-                mbar_arrive(&sm.state_ready[c % 3]);
+                arrive(&sm.state_ready[c % 3]);
                 if (c + 1 < chunks) decay_keys(c + 1);  // their buffer's last reader was done before the state was
             }
         }
@@ -599,7 +616,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
             if constexpr (!kBf16) {
                 const int mine = static_cast<int>(__float_as_uint(most) >> 23);
                 sm.most_p[c & 1][side][row] = static_cast<uint8_t>(mine);
-                mbar_arrive(&sm.most_ready[1]);
+                arrive(&sm.most_ready[1]);
                 if (!wait(&sm.most_ready[1], c)) break;
                 const int2 f = down_and_up(max(mine, static_cast<int>(sm.most_p[c & 1][side ^ 1][row])));
                 down = of_field(f.x);
@@ -617,7 +634,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
             for (int u = 0; u < 4; ++u) *reinterpret_cast<uint4*>(to + (((4 * side + u) ^ (row & 7)) << 4)) = make_uint4(p[4 * u], p[4 * u + 1], p[4 * u + 2], p[4 * u + 3]);
             fence_proxy_async();
             tc::fence_before_sync();
-            mbar_arrive(&sm.p_ready[c & 1]);
+            arrive(&sm.p_ready[c & 1]);
         }
     } else if (!kSums) {
         // ---- row warps: head dim `dim`, 32 tokens (heads of 64 dims, which are there twice: 16), 16 at a time
@@ -642,15 +659,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                 tc::tmem_ld_wait();
                 F2 zeros(0.0f, 0.0f);
 #pragma unroll
-                for (int e = 0; e < kTokens; e += 2) {
-                    const float2 in = kBf16 ? make_float2(V.scale, V.scale) : *reinterpret_cast<const float2*>(&sm.inside[c & 1][i0 + e]);
-                    const float2 before = *reinterpret_cast<const float2*>(&sm.before[i0 + e]);
-                    F2 part = mul2(pair_of_words(s[e], s[e + 1]), F2(before.x, before.y));
-                    if constexpr (!kBf16) part = mul2(part, F2(up, up));
-                    const F2 y = fma2(pair_of_words(r[e], r[e + 1]), F2(in.x, in.y), part);
-                    zeros = fma2(y, F2(0.0f, 0.0f), zeros);
-                    r[e] = __float_as_uint(y.get().x);
-                    r[e + 1] = __float_as_uint(y.get().y);
+                for (int e = 0; e < kTokens; e += 4) {
+                    const float4 in = kBf16 ? make_float4(V.scale, V.scale, V.scale, V.scale) : *reinterpret_cast<const float4*>(&sm.inside[c & 1][i0 + e]);
+                    const float4 before = *reinterpret_cast<const float4*>(&sm.before[i0 + e]);
+#pragma unroll
+                    for (int h = 0; h < 4; h += 2) {
+                        F2 part = mul2(pair_of_words(s[e + h], s[e + h + 1]), h ? F2(before.z, before.w) : F2(before.x, before.y));
+                        if constexpr (!kBf16) part = mul2(part, F2(up, up));
+                        const F2 y = fma2(pair_of_words(r[e + h], r[e + h + 1]), h ? F2(in.z, in.w) : F2(in.x, in.y), part);
+                        zeros = fma2(y, F2(0.0f, 0.0f), zeros);
+                        r[e + h] = __float_as_uint(y.get().x);
+                        r[e + h + 1] = __float_as_uint(y.get().y);
+                    }
                 }
                 if (!(zeros.get().x + zeros.get().y == 0.0f)) {
 #pragma unroll 1
@@ -672,13 +692,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                 __syncwarp();
                 if (b == kBlocks - 1) {
                     tc::fence_before_sync();
-                    mbar_arrive(&sm.out_read[c & 1]);
+                    arrive(&sm.out_read[c & 1]);
                 }
                 uint32_t* const out = sm.out[c & 1] + i0 / 2 * D + dim;
 #pragma unroll
                 for (int e = 0; e < kTokens / 2; ++e) out[e * D] = pack_pair<kBf16>(pair_of_words(r[2 * e], r[2 * e + 1]));
             }
-            mbar_arrive(&sm.out_ready[c & 1]);
+            arrive(&sm.out_ready[c & 1]);
         }
     }
     if (failed && lane == 0 && V.error_word != nullptr) atomicOr(V.error_word, KVB_ERR_WAIT_TIMEOUT);
