@@ -27,7 +27,8 @@ namespace {
 constexpr int kStepThreads = 256;
 
 // One CTA has kCols columns of the state of one sequence and head, in registers, for all tokens of the sequence; thread (row group, four columns).  The
-// rows of q, k (whole) and v (its columns) of a token go through shared memory; the sums over the state's rows by shuffles, then shared memory.
+// rows of q, k (whole) and v (its columns) of a token go through shared memory, asked for a token ahead; the sums over the state's rows by shuffles, then
+// shared memory.
 template <int D, int kCols, bool kBf16>
 __global__ void __launch_bounds__(kStepThreads) step_kernel(LinearView L) {
     constexpr int kVecs = kCols / 4, kGroups = kStepThreads / kVecs, kRows = D / kGroups;
@@ -48,13 +49,26 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(LinearView L) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r) S[r] = *reinterpret_cast<const float4*>(from + (group + r * kGroups) * D);
     const int qk_head = head / L.share;
+    constexpr int kEach = (2 * D + kCols + kStepThreads - 1) / kStepThreads;  // elements of a token's rows, a thread
+    uint16_t row[kEach];
+    auto ask = [&](int64_t t) {
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) {
+            const int i = tid + n * kStepThreads;
+            if (i < D) row[n] = L.q[t * L.q_stride + qk_head * D + i];
+            else if (i < 2 * D) row[n] = L.k[t * L.k_stride + qk_head * D + i - D];
+            else if (i < 2 * D + kCols) row[n] = L.v[t * L.v_stride + head * D + col0 + i - 2 * D];
+        }
+    };
+    if (s.begin < s.end) ask(s.begin);
     for (int t = s.begin; t < s.end; ++t) {
-        for (int i = tid; i < 2 * D + kCols; i += kStepThreads) {
-            if (i < D) qs[i] = in_to_f32<kBf16>(L.q[t * L.q_stride + qk_head * D + i]);
-            else if (i < 2 * D) ks[i - D] = in_to_f32<kBf16>(L.k[t * L.k_stride + qk_head * D + i - D]);
-            else vs[i - 2 * D] = in_to_f32<kBf16>(L.v[t * L.v_stride + head * D + col0 + i - 2 * D]);
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) {
+            const int i = tid + n * kStepThreads;
+            if (i < 2 * D + kCols) (i < D ? qs[i] : i < 2 * D ? ks[i - D] : vs[i - 2 * D]) = in_to_f32<kBf16>(row[n]);
         }
         __syncthreads();
+        if (t + 1 < s.end) ask(t + 1);
         const float4 v = make_float4(vs[4 * vec], vs[4 * vec + 1], vs[4 * vec + 2], vs[4 * vec + 3]);
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
@@ -135,7 +149,13 @@ int linear_call(const kvb_linear* layer, const char* who, const void* q, int64_t
     V.head_dim = D;
     V.error_word = layer->error_word;
     const bool bf = layer->dtype == KVB_DTYPE_BF16;
-    if (static_cast<int64_t>(tokens) > 16 * static_cast<int64_t>(batch)) {
+    // Few tokens a sequence go one after another (verify steps of up to eight rows always): a token costs 0.4 .. 1.1 us, by how many heads and
+    // sequences share the device, a call of the chunked form 7 us (64 dims) or 10 a wave of its CTAs, one an SM.  Measured on B200, 32 value heads, us one
+    // after another / in chunks at the tokens where they meet: 64 dims 1 sequence 12 6.9 / 6.9, 2 8 7.2 / 6.9, 4 5 7.2 / 7.3, 8 8 13.0 / 13.3; 128 dims 1
+    // 17 9.0 / 10.0, 2 11 10.3 / 10.3, 4 7 10.6 / 10.6, 8 10 22.5 / 22.6, 16 12 44.2 / 43.7.  The lines between them lie within 2.5 us of the better form.
+    const int64_t units = static_cast<int64_t>(batch) * layer->v_heads, sms = device_sm_count();
+    const int few = units <= sms / 3 ? 12 : units <= sms ? 8 : 10;
+    if (offsets != nullptr && static_cast<int64_t>(tokens) > static_cast<int64_t>(few) * batch) {
         if (workspace == nullptr) return fail(KVB_EINVAL, "%s: null workspace", who);
         const bool aligned = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) == 0 && q_stride % 8 == 0 && k_stride % 8 == 0 && v_stride % 8 == 0;
         return linear_chunks(V, bf, aligned, workspace, stream);
