@@ -57,11 +57,11 @@ template <int D> struct LinearSmem {
     uint32_t out[2][kTileBytes / 4];       // outputs of two chunks, [32 pairs of tokens][D]
     float fade[2][2 * kC + 16];            // fade[s][x] = lambda^(63 - x - s), 0 behind lambda^0; the second copy for aligned pairs from odd x on, 16 banks further
     alignas(16) float before[kC];                      // scale lambda^(i + 1)
-    float inside[2][kC];                   // scale times what P's row i was scaled down by (fp16)
+    uint8_t inside[2][kC];                 // exponent field of what P's row i was scaled down by (fp16)
     uint8_t up[3][128];                    // exponent field of what a row of the state was scaled down by (fp16)
     uint8_t most_state[2][128], most_p[2][2][kC];  // exponents of the largest magnitudes of a row, one a column half (fp16)
-    // chunk c has the one of c mod their number; done: the state's products of a chunk; rows_done: P V of chunk c - 2 and the scores of chunk c
-    uint64_t full[kStages], done[kStages], rows_done[kStages], state_ready[3], p_ready[2], keys_ready[2], out_read[2], out_ready[2], out_free[2], most_ready[2], loaded, drained[2];
+    // chunk c has the one of c mod their number; done: the state's products of a chunk; rows_done: its P V; scores: its scores
+    uint64_t full[kStages], done[kStages], rows_done[kStages], scores[kStages], state_ready[3], p_ready[2], keys_ready[2], out_read[2], out_ready[2], out_free[2], most_ready[2], loaded, drained[2];
     uint32_t tmem_base;
     int abort_flag;
     int unit[3];
@@ -255,6 +255,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
             mbar_init(&sm.full[s], 1);
             mbar_init(&sm.done[s], 1);
             mbar_init(&sm.rows_done[s], 1);
+            mbar_init(&sm.scores[s], 1);
             mbar_init(&sm.state_ready[s], kStateWarps);
         }
         for (int s = 0; s < 2; ++s) {
@@ -345,7 +346,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
             typename Smem::Stage& st = sm.stage[stage];
             const int64_t t = begin + c * kC;
             // the products of the stage's chunk before: the state's, its P V
-            if (c >= kStages && (!wait3(sm.done, c - kStages) || (!kSums && !wait3(sm.rows_done, c - kStages + 2)))) break;
+            if (c >= kStages && (!wait3(sm.done, c - kStages) || (!kSums && !wait3(sm.rows_done, c - kStages)))) break;
             if (P.aligned) {
                 if (lane == 0) {
                     mbar_expect_tx(&sm.full[stage], (kSums ? 2 : 3) * Smem::kTileBytes);
@@ -378,7 +379,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
             uint16_t* const to = V.out + (t * V.v_heads + head) * D;
             const uint32_t* const words = sm.out[c & 1];  // of a head dim and two tokens
             if (wide) {
-                constexpr int kUnits = D / 8, kAtOnce = 4;  // 8 dims a unit
+                constexpr int kUnits = D / 8, kAtOnce = 2;  // 8 dims a unit; bursts of stores are in everybody's way
 #pragma unroll 1
                 for (int u0 = lane; u0 < kC / 2 * kUnits; u0 += 32 * kAtOnce) {
                     uint4 r[kAtOnce][2];
@@ -444,6 +445,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                         const uint64_t a = dims_desc(sm.stage[c % kStages].v), b = rows_desc(sm.p[c & 1]);
 #pragma unroll
                         for (int s = 0; s < kC / 16; ++s) tc::mma_f16_ss(tmem + kInsideCol, tc::desc_at(a, s * 2048), k_major(b, s), kOut, s > 0);
+                        tc::commit(&sm.rows_done[c % 3]);
                     }
                     __syncwarp();
                 }
@@ -454,11 +456,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                         const uint64_t a = rows_desc(sm.stage[n % kStages].q), b = rows_desc(sm.stage[n % kStages].k);
 #pragma unroll
                         for (int s = 0; s < D / 16; ++s) tc::mma_f16_ss(tmem + kScoreCol + (n & 1) * kC, k_major(a, s), k_major(b, s), kScores, s > 0);
+                        tc::commit(&sm.scores[n % 3]);
                     }
                     __syncwarp();
                 }
-                if (tc::elect_one()) tc::commit(&sm.rows_done[n % 3]);
-                __syncwarp();
             }
         }
         if (failed) {  // nothing is freed under MMAs that still run
@@ -476,7 +477,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
         // decayed keys of chunk c, two numbers each
         auto decay_keys = [&](int c) {
             if (!wait3(sm.full, c)) return;
-            if (!kSums && !wait3(sm.rows_done, c)) return;  // the keys themselves have been read
+            if (!kSums && !wait3(sm.scores, c)) return;  // the keys themselves have been read
             const int t = begin + c * kC, valid = min(kC, end - t);
             unsigned char* const keys = sm.stage[c % kStages].k;
             unsigned char* const second = sm.second[c & 1];
@@ -601,7 +602,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
         // ---- score warps: rows 0 .. 63 of the scores, 32 columns a warp
         const int quad = warp & 3, side = (warp - kLastWarps) >> 2, row = 32 * quad + lane, j0 = 32 * side;
         for (int c = 0; c < chunks; ++c) {
-            if (!wait3(sm.rows_done, c)) break;
+            if (!wait3(sm.scores, c)) break;
             tc::fence_after_sync();
             uint32_t s[32], p[16];
             float most = 0.0f;
@@ -623,7 +624,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
 #pragma unroll
                 for (int e = 0; e < 32; ++e) s[e] = 0u;
             }
-            float down = 1.0f, up = 1.0f;
+            float down = 1.0f;
+            int up = 0;
             if constexpr (!kBf16) {
                 const int mine = static_cast<int>(__float_as_uint(most) >> 23);
                 sm.most_p[c & 1][side][row] = static_cast<uint8_t>(mine);
@@ -631,7 +633,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                 if (!wait(&sm.most_ready[1], c)) break;
                 const int2 f = down_and_up(max(mine, static_cast<int>(sm.most_p[c & 1][side ^ 1][row])));
                 down = of_field(f.x);
-                up = of_field(f.y);
+                up = f.y;
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -639,7 +641,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                 p[e] = pack_pair<kBf16>(kBf16 ? x : mul2(x, F2(down, down)));
             }
             if (c > 1 && !wait2(sm.out_read, c - 2)) break;  // nobody looks at P of the chunk before the last, and its scales, any more
-            if (!kBf16 && side == 0) sm.inside[c & 1][row] = V.scale * up;
+            if (!kBf16 && side == 0) sm.inside[c & 1][row] = static_cast<uint8_t>(up);
             unsigned char* const to = sm.p[c & 1] + row * 128;
 #pragma unroll
             for (int u = 0; u < 4; ++u) *reinterpret_cast<uint4*>(to + (((4 * side + u) ^ (row & 7)) << 4)) = make_uint4(p[4 * u], p[4 * u + 1], p[4 * u + 2], p[4 * u + 3]);
@@ -656,7 +658,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
         for (int c = 0; c < chunks; ++c) {
             const int64_t t = begin + c * kC;
             const int valid = min(kC, end - static_cast<int>(t));
-            if (!wait3(sm.done, c) || !wait3(sm.rows_done, c + 2)) break;
+            if (!wait3(sm.done, c) || !wait3(sm.rows_done, c)) break;
             if (!kBf16 && (!wait3(sm.state_ready, c) || !wait2(sm.p_ready, c))) break;  // sm.up, sm.inside of all rows
             if (c > 1 && !wait2(sm.out_free, c - 2)) break;
             tc::fence_after_sync();
@@ -671,7 +673,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                 F2 zeros(0.0f, 0.0f);
 #pragma unroll
                 for (int e = 0; e < kTokens; e += 4) {
-                    const float4 in = kBf16 ? make_float4(V.scale, V.scale, V.scale, V.scale) : *reinterpret_cast<const float4*>(&sm.inside[c & 1][i0 + e]);
+                    float4 in = make_float4(V.scale, V.scale, V.scale, V.scale);
+                    if constexpr (!kBf16) {
+                        const uchar4 f = *reinterpret_cast<const uchar4*>(&sm.inside[c & 1][i0 + e]);
+                        in = make_float4(V.scale * of_field(f.x), V.scale * of_field(f.y), V.scale * of_field(f.z), V.scale * of_field(f.w));
+                    }
                     const float4 before = *reinterpret_cast<const float4*>(&sm.before[i0 + e]);
 #pragma unroll
                     for (int h = 0; h < 4; h += 2) {
@@ -692,7 +698,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                         for (int x = 0; x < kTokens; ++x)
                             if (x == e) word = r[x], part = s[x];
                         if ((word & 0x7F800000u) != 0x7F800000u || i >= valid) continue;
-                        const float in = kBf16 ? V.scale : sm.inside[c & 1][i];
+                        const float in = kBf16 ? V.scale : V.scale * of_field(sm.inside[c & 1][i]);
                         const float again = inside_again<kBf16>(sm.p[c & 1], i, V.v + t * V.v_stride + head * D + dim, V.v_stride);
                         const float y = fmaf(again, in, __uint_as_float(part) * sm.before[i] * up);
 #pragma unroll
