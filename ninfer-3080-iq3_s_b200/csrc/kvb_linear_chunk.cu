@@ -42,7 +42,7 @@ constexpr int kStages = 3;
 constexpr int kStateWarps = 8, kRowWarps = 8;
 // the last eight: warps 0, 1, 4, 5 of them P (rows 0 .. 63 of tensor memory are a warp's by its number mod 4)
 constexpr int kLastWarps = kStateWarps + kRowWarps, kStateMmaWarp = kLastWarps + 2, kLoadWarp = kLastWarps + 3, kRowMmaWarp = kLastWarps + 6, kStoreWarp = kLastWarps + 7;
-constexpr int kStateThreads = kStateWarps * 32, kScoreWarps = 4;
+constexpr int kScoreWarps = 4;
 constexpr int kChunkThreads = (kLastWarps + 8) * 32;  // 24 warps: six to a scheduler, 80 registers a thread
 constexpr uint32_t kTmemCols = 512;
 
@@ -220,7 +220,8 @@ template <bool kBf16> __device__ __noinline__ float inside_again(const unsigned 
 template <int D, bool kBf16, bool kSums>
 __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_constant__ ChunkCall P) {
     using Smem = LinearSmem<D>;
-    constexpr int kHalf = D / 2;  // columns of the state a state warp has
+    // in the first launch the row warps help with the keys
+    constexpr int kKeyWarps = kSums ? kLastWarps : kStateWarps, kKeyThreads = kKeyWarps * 32, kHalf = 4 * D / kKeyWarps;  // kHalf: columns of the state such a warp has
     constexpr uint32_t kStateCol = 0, kOperandCol = D, kScoreCol = D + D / 2, kBeforeCol = kScoreCol + 2 * kC, kInsideCol = kBeforeCol + 2 * kC;
     static_assert(kInsideCol + kC <= kTmemCols, "tensor memory");
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(&sm.p_ready[s], kScoreWarps);
-            mbar_init(&sm.keys_ready[s], kStateWarps);
+            mbar_init(&sm.keys_ready[s], kKeyWarps);
             mbar_init(&sm.out_read[s], kRowWarps);
             mbar_init(&sm.out_ready[s], kRowWarps);
             mbar_init(&sm.out_free[s], 1);
@@ -468,7 +469,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
             __syncwarp();
             mbar_wait_bounded(drained, 0);
         }
-    } else if (warp < kStateWarps) {
+    } else if (warp < kKeyWarps) {
         // ---- state warps: rows 32 (warp % 4) + lane of S^T, columns by warp / 4
         const int quad = warp & 3, side = warp >> 2, row = 32 * quad + lane, dim = row % D, tid = threadIdx.x;
         const uint32_t lanes = static_cast<uint32_t>(32 * quad) << 16;
@@ -481,10 +482,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
             const int t = begin + c * kC, valid = min(kC, end - t);
             unsigned char* const keys = sm.stage[c % kStages].k;
             unsigned char* const second = sm.second[c & 1];
-            constexpr int kEach = kC * D / 8 / kStateThreads;
+            constexpr int kEach = kC * D / 8 / kKeyThreads;
 #pragma unroll
             for (int n = 0; n < kEach; ++n) {
-                const int u = tid + n * kStateThreads, j = (u >> 3) & (kC - 1);
+                const int u = tid + n * kKeyThreads, j = (u >> 3) & (kC - 1);
                 const float w = kSums ? decay_power(g, end - 1 - t - j) : sm.fade[0][kC - 1 - max(valid - 1 - j, 0)];
                 uint4 raw = *reinterpret_cast<const uint4*>(keys + 16 * u);
                 if (j >= valid) raw = make_uint4(0u, 0u, 0u, 0u);
@@ -512,7 +513,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                 *reinterpret_cast<uint4*>(second + 16 * u) = make_uint4(b[0], b[1], b[2], b[3]);
             }
             if (valid < kC) {  // values behind the sequence's last row meet zeros in P and the keys: they have to be finite
-                for (int u = tid; u < kC * D / 8; u += kStateThreads)
+                for (int u = tid; u < kC * D / 8; u += kKeyThreads)
                     if (((u >> 3) & (kC - 1)) >= valid) *reinterpret_cast<uint4*>(sm.stage[c % kStages].v + 16 * u) = make_uint4(0u, 0u, 0u, 0u);
             }
             fence_proxy_async();
