@@ -775,6 +775,7 @@ extern "C" int kvb_rope_append(const kvb_layer* layer, const kvb_rope* rope, con
     if (q != nullptr) {
         R.wide_q = rope_is_wide(*rope, D, q, q_out, q_stride, q_out_stride);
         R.q = rope_rows_of(*rope, q, q_out, positions_dev, tokens, layer->q_heads, D, q_stride, q_out_stride, R.wide_q);
+        R.q.in_a_row = tokens;
     }
     const LayerView V = make_view(*layer);
     cudaStream_t s = static_cast<cudaStream_t>(stream);

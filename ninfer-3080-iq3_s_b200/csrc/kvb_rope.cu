@@ -10,6 +10,7 @@ namespace kvb {
 
 int check_rope(const kvb_rope* rope, int head_dim, const char* who) {
     if (rope == nullptr || rope->inv_freq == nullptr) return fail(KVB_EINVAL, "%s: null rope / inv_freq", who);
+    if ((reinterpret_cast<uintptr_t>(rope->inv_freq) & 7u) != 0) return fail(KVB_EINVAL, "%s: inv_freq starts at an 8-byte boundary", who);
     if (rope->rotary_dim < 2 || rope->rotary_dim % 2 != 0 || rope->rotary_dim > head_dim)
         return fail(KVB_EINVAL, "%s: rotary_dim %d must be even, 2..head_dim (%d)", who, rope->rotary_dim, head_dim);
     if (rope->interleaved != 0 && rope->interleaved != 1) return fail(KVB_EINVAL, "%s: interleaved = %d", who, rope->interleaved);
@@ -28,6 +29,7 @@ RopeRows rope_rows_of(const kvb_rope& rope, const void* x, void* out, const int3
     P.out_stride = out_stride;
     P.heads = heads;
     P.head_dim = head_dim;
+    P.in_a_row = 0;
     const int turning = wide ? (rope.interleaved ? rope.rotary_dim / 8 : rope.rotary_dim / 16) : rope.rotary_dim / 2;
     const int passing = x == out ? 0 : (head_dim - rope.rotary_dim) / (wide ? 8 : 1);  // in place they are there already
     P.units = turning + passing;
@@ -45,7 +47,12 @@ template <bool kBf16, bool kWide> __global__ void __launch_bounds__(kRopeThreads
     if (!beside) grid_dependency_wait();
     launch_dependents();
     const int64_t item = static_cast<int64_t>(blockIdx.x) * kRopeThreads + threadIdx.x;
-    if (item < P.items) rope_item<kBf16, kWide>(P, item);
+    bool sound = true;
+    if (P.in_a_row > 0) {
+        const int first = P.positions[0], last = P.positions[P.in_a_row - 1];
+        sound = first >= 0 && last - first == P.in_a_row - 1;
+    }
+    if (sound && item < P.items) rope_item<kBf16, kWide>(P, item);
     if (beside) grid_dependency_wait();  // nobody leaves before the append is over: what waits for this grid finds both done
 }
 

@@ -50,6 +50,7 @@ struct RopeRows {
     const int32_t* positions;
     int64_t x_stride, out_stride, items;
     int heads, head_dim, units, splits;
+    int in_a_row;  // that many positions have to follow one another from 0 or more on, or nothing is written; 0: any positions
 };
 
 template <bool kBf16> __device__ __forceinline__ void unpack8_16(uint4 v, float (&f)[8]) {

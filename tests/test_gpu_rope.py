@@ -227,6 +227,36 @@ def test_append_leaves_everything_where_positions_are_refused():
     assert bool((out == 7).all()) and not layer.stage.any() and not layer.k_code.any() and not layer.v_scale.any()
 
 
+@pytest.mark.parametrize("start,T", [(0, 600), (100, 900)])
+def test_queries_beside_the_append(start, T):
+    """So many tiles that the queries are a launch of their own, which starts beside the append: the same queries and cache, and nothing written where the positions
+    are refused; what comes next in the stream finds both done."""
+    import torch
+
+    D, H, QH = 256, 8, 40
+    g = torch.Generator(device="cuda").manual_seed(T)
+    k, v, q = (torch.randn((T, n, D), generator=g, device="cuda").bfloat16() for n in (H, H, QH))
+    pos = torch.arange(start, start + T, dtype=torch.int32, device="cuda")
+    rope = _rope(64, base=1e6)
+    one = _layer(D, H, QH, start + T, "bf16")
+    one.rope_append(rope, k, v, pos)
+    want = rope.rows(q, pos)
+    for _ in range(3):
+        two = _layer(D, H, QH, start + T, "bf16")  # a new one: an append that begins inside a tile finds other rows there after one that passed it
+        mine = q.clone()
+        got = two.rope_append(rope, k, v, pos, q=mine, q_out=mine)
+        rows = two.read_rows(start, T, pos[-1:])
+        assert torch.equal(got, want) and _same(one, two)
+        assert all(torch.equal(a, b) for a, b in zip(rows, one.read_rows(start, T, pos[-1:])))
+    assert two.errors() == 0
+    for bad in (pos.flip(0).contiguous(), pos - start - 1):
+        out = torch.full_like(q, 7)
+        two.error_word.zero_()
+        two.rope_append(rope, k, v, bad, q=q, q_out=out)
+        assert two.errors() == pkg().capi.ERR_POSITIONS
+        assert bool((out == 7).all()) and _same(one, two)
+
+
 def test_steps_and_prompts_over_turned_keys():
     """As an engine uses them: a prompt turned with kvb_rope_rows and prefilled, then decode steps whose append turns the key; against attention in 64 bits over
     the same rows.  Tolerance: K and V in 4 bits.  A step of a row's codes is (hi - lo) / 15, a value is off by half of one at most; for rows of

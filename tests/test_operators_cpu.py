@@ -85,7 +85,7 @@ def test_rope_rows_refused():
         return lib.kvb_rope_rows(None if R is None else C.byref(R), x, xs, out, os, pos, tokens, heads, dim, dtype, None)
 
     assert call(tokens=0) == capi.KVB_OK
-    for bad in (dict(R=None), dict(R=_rope(capi, inv_freq=None)), dict(R=_rope(capi, rotary_dim=63)), dict(R=_rope(capi, rotary_dim=0)), dict(R=_rope(capi, rotary_dim=130)),
+    for bad in (dict(R=None), dict(R=_rope(capi, inv_freq=None)), dict(R=_rope(capi, inv_freq=(1 << 20) + 4)), dict(R=_rope(capi, rotary_dim=63)), dict(R=_rope(capi, rotary_dim=0)), dict(R=_rope(capi, rotary_dim=130)),
                 dict(R=_rope(capi, interleaved=2)), dict(R=_rope(capi, factor=math.nan)), dict(x=None), dict(out=None), dict(pos=None), dict(tokens=-1), dict(heads=0), dict(dim=0),
                 dict(dtype=2), dict(xs=1023), dict(os=1000),
                 dict(out=16 * MIB + 16),             # beside x, not x itself
