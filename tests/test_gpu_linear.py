@@ -339,3 +339,103 @@ def test_slots_far_into_the_pool():
         o, oo, s, so = _wanted(layer, q[rows], k[rows], v[rows], 0.1, before[b])
         _close(out[rows], o, oo, f"out {b}")
         _close(layer.state[at[b]], s, so, f"state {b}")
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lengths", [[200, 3, 77], [450]])
+def test_rows_at_any_boundary(dtype, D, lengths):
+    """Rows that start off the 16-byte boundary, and rows an odd number of elements apart: the bits of packed ones."""
+    import torch
+
+    n, tokens, qk, vh = len(lengths), sum(lengths), 40, 80
+    q, k, v = (x.contiguous() for x in _inputs(qk, vh, D, tokens, dtype, tokens))
+    offsets, slots = _i32([sum(lengths[:b]) for b in range(n + 1)]), _i32(list(range(n)))
+
+    def call(q, k, v):
+        layer = _layer(qk, vh, D, n, dtype)
+        _fill(layer, 5)
+        out = layer.chunk(q, k, v, offsets, D ** -0.5, slots, slots)
+        assert layer.errors() == 0
+        return out, layer.state
+
+    def moved(x, shift, gap):
+        stride = x[0].numel() + gap
+        buf = torch.zeros(tokens * stride + shift, dtype=x.dtype, device="cuda")
+        y = buf[shift:].as_strided(x.shape, (stride, D, 1))
+        y.copy_(x)
+        return y
+
+    want = call(q, k, v)
+    for shift, gap in ((1, 0), (0, 3), (3, 8), (8, 8)):
+        got = call(moved(q, shift, gap), moved(k, shift, gap), moved(v, shift, gap))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), (shift, gap)
+
+
+@pytest.mark.parametrize("longest", [8, 60, 300])
+def test_as_many_sequences_as_a_call_takes(longest):
+    import random
+
+    import torch
+
+    D, vh, rng = 64, 2, random.Random(longest)
+    lengths = [rng.randint(0, longest) for _ in range(256)]
+    tokens = sum(lengths)
+    layer = _layer(1, vh, D, 256, "bf16")
+    before = _fill(layer, 1)
+    q, k, v = _inputs(1, vh, D, tokens, "bf16", 3)
+    slots = torch.randperm(256, generator=torch.Generator().manual_seed(1)).tolist()
+    offsets = [sum(lengths[:b]) for b in range(257)]
+    out = layer.chunk(q, k, v, _i32(offsets), 0.2, _i32(slots), _i32(slots))
+    assert layer.errors() == 0
+    for b in range(0, 256, 1 if longest < 100 else 17):
+        rows = slice(offsets[b], offsets[b + 1])
+        if not lengths[b]:
+            assert torch.equal(layer.state[slots[b]], before[slots[b]])
+            continue
+        o, oo, s, so = _wanted(layer, q[rows], k[rows], v[rows], 0.2, before[slots[b]])
+        _close(out[rows], o, oo, f"out {b}")
+        _close(layer.state[slots[b]], s, so, f"state {b}")
+
+
+def test_two_streams_at_once():
+    """Calls of two layers on two streams, each with its own workspace: the bits of one after the other."""
+    import torch
+
+    sets = []
+    for i in range(2):
+        layer = _layer(2, 4, 128, 2, "bf16")
+        first = _fill(layer, i)
+        q, k, v = _inputs(2, 4, 128, 3000, "bf16", 10 + i)
+        sets.append((layer, first, q, k, v))
+    off, r, w = _i32([0, 3000]), _i32([0]), _i32([1])
+    want = []
+    for layer, first, q, k, v in sets:
+        out = layer.chunk(q, k, v, off, 0.1, r, w)
+        want.append((out.clone(), layer.state.clone()))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        got = []
+        for (layer, first, q, k, v), stream in zip(sets, streams):
+            layer.state[1].zero_()
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                got.append(layer.chunk(q, k, v, off, 0.1, r, w))
+        torch.cuda.synchronize()
+        for (layer, *_), g, (out, state) in zip(sets, got, want):
+            assert torch.equal(g, out) and torch.equal(layer.state, state) and layer.errors() == 0
+
+
+def test_same_inputs_same_bits():
+    """No sum depends on which CTA or warp comes first."""
+    import torch
+
+    layer = _layer(4, 8, 64, 6, "fp16")
+    first = _fill(layer, 2)
+    q, k, v = _inputs(4, 8, 64, 2000, "fp16", 6)
+    args = (q, k, v, _i32([0, 900, 901, 2000]), 0.1, _i32([0, 1, 2]), _i32([3, 4, 5]))
+    out, state = layer.chunk(*args).clone(), layer.state.clone()
+    for _ in range(5):
+        layer.state.copy_(first)
+        assert torch.equal(layer.chunk(*args), out) and torch.equal(layer.state, state)

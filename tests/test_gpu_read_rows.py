@@ -102,3 +102,30 @@ def test_rows_behind_the_newest_and_bad_pages_stay():
     layer.read_rows(0, n, torch.tensor([n - 1], dtype=torch.int32, device="cuda"), *outs)
     assert layer.errors() == pkg().capi.ERR_TABLE_RANGE
     assert bool((outs[0][256:384] == 7).all()) and torch.equal(outs[0][:256], full[0][:256])
+
+
+@pytest.mark.parametrize("D", [128, 256])
+def test_outputs_at_16_bytes_captured_and_on_another_stream(D):
+    import torch
+
+    n = 900
+    tw = Twin(D=D, H=2, QH=4, capacity_tokens=n, seed=4, dtype=1)
+    tw.append(*(orc.synth_kv(1, n, 2, D, i) for i in (1, 2)))
+    layer, pos = tw.gpu, torch.tensor([n - 1], dtype=torch.int32, device="cuda")
+    want = layer.read_rows(37, 800, pos)
+    bufs = [torch.full((800 * 2 * D + 16,), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    outs = [b[8:8 + 800 * 2 * D].view(800, 2, D) for b in bufs]  # 16 bytes further
+    assert outs[0].data_ptr() % 32 == 16
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            layer.read_rows(37, 800, pos, *outs)
+    for _ in range(2):
+        for o in outs:
+            o.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+        assert all(bool((b[:8] == 7).all()) and bool((b[-8:] == 7).all()) for b in bufs)
+    assert layer.errors() == 0
