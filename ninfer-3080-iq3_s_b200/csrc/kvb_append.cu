@@ -522,8 +522,10 @@ struct AppendRope {
     bool wide_k, wide_v, wide_q;
 };
 struct NoRope {};
-template <int D, bool kBf16, bool kRope>
-__global__ void __launch_bounds__(kThreads, 1) append_kernel(LayerView L, const uint16_t* __restrict__ k,
+// kBalances = false: the form for layers without balancing, whose CTA leaves registers of its SM to CTAs that turn queries beside it.
+constexpr int kLeanBound = 640;  // as a bound of the CTA's threads: 96 registers a thread
+template <int D, bool kBf16, bool kRope, bool kBalances>
+__global__ void __launch_bounds__(kBalances ? kThreads : kLeanBound, 1) append_kernel(LayerView L, const uint16_t* __restrict__ k,
                                                              const uint16_t* __restrict__ v,
                                                              const int32_t* __restrict__ positions, int tokens, std::conditional_t<kRope, AppendRope, NoRope> R) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -610,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1) append_kernel(LayerView L, const 
     float x[kPer];  // along the rows of the matrix
     if (which) load_by_token(sm, x);
     else load_by_dim(sm, x);
-    if (L.iters > 0) {
+    if (kBalances && L.iters > 0) {
         float y[kPer];  // along its columns
         if (which) {
             load_by_dim(sm, y);
@@ -695,28 +697,30 @@ int launch_append(const LayerView& V, const void* k, const void* v, const int32_
     static_assert(sizeof(AppendSmem) <= 227 * 1024, "shared memory");
     static OncePerDevice opted;  // per template instance
     const int smem = static_cast<int>(sizeof(AppendSmem));
-    KVB_CUDA_OK(allow_smem(opted, append_kernel<D, kBf16, false>, smem));
+    KVB_CUDA_OK(allow_smem(opted, append_kernel<D, kBf16, false, true>, smem));
     const dim3 grid(tokens / kTile + 2, V.kv_heads, 2 * Geo<D>::S);
-    KVB_CUDA_OK(launch_early(append_kernel<D, kBf16, false>, grid, dim3(kThreads), smem, stream, V, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
+    KVB_CUDA_OK(launch_early(append_kernel<D, kBf16, false, true>, grid, dim3(kThreads), smem, stream, V, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
                              positions, tokens, NoRope{}));
     return KVB_OK;
 }
 
-template <int D, bool kBf16>
+template <int D, bool kBf16, bool kBalances>
 int launch_rope_append(const LayerView& V, AppendRope R, const void* k, const void* v, const int32_t* positions, int tokens, cudaStream_t stream) {
     constexpr int most = static_cast<int>(sizeof(AppendSmem)) + rope_bytes(D, kTile);
     static_assert(sizeof(AppendSmem) % 16 == 0 && most <= 227 * 1024, "shared memory");
     static OncePerDevice opted;  // per template instance
-    KVB_CUDA_OK(allow_smem(opted, append_kernel<D, kBf16, true>, most));
+    KVB_CUDA_OK(allow_smem(opted, append_kernel<D, kBf16, true, kBalances>, most));
     R.tiles = tokens / kTile + 2;
     const int smem = static_cast<int>(sizeof(AppendSmem)) + rope_bytes(R.rope.rotary, tokens < kTile ? tokens : kTile);
     // The queries are the same launch's where all of its CTAs are resident at once (one an SM), in whole columns of the grid; else a launch beside it,
-    // whose smaller CTAs take the SMs that the append leaves.  Measured on B200, 1,024 tokens of 4 and 24 heads of 256 dims: 20.8 us as one launch, 19.6 as two.
+    // whose smaller CTAs take the SMs that the append leaves, and what registers the form without balancing leaves on its own.  Measured on B200, graph
+    // replay, 4 and 24 heads of 256 dims: 1,024 tokens 20.8 us as one launch, 17.5 as two, 16.5 with the lean form; 777 tokens 15.0 as two, 12.6 with the
+    // lean form, 11.3 the keys alone.  Of 128 dims, 1,300 tokens: 11.8 as two, 9.4 with the lean form (777 tokens 9.0 and 9.4; keys alone 8.3 ... 8.6).
     const int column = V.kv_heads * 2 * Geo<D>::S;
     const int64_t ctas = R.q.x == nullptr ? 0 : (R.q.items + kThreads - 1) / kThreads, columns = (ctas + column - 1) / column;
     const bool beside = (R.tiles + columns) * column > device_sm_count();
     const dim3 grid(R.tiles + (beside ? 0 : static_cast<unsigned>(columns)), V.kv_heads, 2 * Geo<D>::S);
-    KVB_CUDA_OK(launch_early(append_kernel<D, kBf16, true>, grid, dim3(kThreads), smem, stream, V, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
+    KVB_CUDA_OK(launch_early(append_kernel<D, kBf16, true, kBalances>, grid, dim3(kThreads), smem, stream, V, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
                              positions, tokens, R));
     return beside && ctas > 0 ? launch_rope(R.q, kBf16, R.wide_q, true, stream) : KVB_OK;
 }
@@ -780,8 +784,12 @@ extern "C" int kvb_rope_append(const kvb_layer* layer, const kvb_rope* rope, con
     const LayerView V = make_view(*layer);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool bf = layer->dtype == KVB_DTYPE_BF16;
-    if (D == 128) return bf ? launch_rope_append<128, true>(V, R, k, v, positions_dev, tokens, s) : launch_rope_append<128, false>(V, R, k, v, positions_dev, tokens, s);
-    return bf ? launch_rope_append<256, true>(V, R, k, v, positions_dev, tokens, s) : launch_rope_append<256, false>(V, R, k, v, positions_dev, tokens, s);
+    auto launch = [&](auto balances) {
+        constexpr bool kBalances = decltype(balances)::value;
+        if (D == 128) return bf ? launch_rope_append<128, true, kBalances>(V, R, k, v, positions_dev, tokens, s) : launch_rope_append<128, false, kBalances>(V, R, k, v, positions_dev, tokens, s);
+        return bf ? launch_rope_append<256, true, kBalances>(V, R, k, v, positions_dev, tokens, s) : launch_rope_append<256, false, kBalances>(V, R, k, v, positions_dev, tokens, s);
+    };
+    return layer->sinkhorn_iters > 0 ? launch(std::true_type{}) : launch(std::false_type{});
 }
 
 extern "C" int kvb_decode_tile(const kvb_layer* layer, int tile, int head, void* out_k, void* out_v, void* stream) {
