@@ -279,7 +279,7 @@ int kvb_rope_frequencies(int rotary_dim, double base, int scaling, double factor
 int kvb_rope_rows(const kvb_rope* rope, const void* x, int64_t x_stride, void* out, int64_t out_stride, const int32_t* positions_dev, int tokens, int heads,
                   int head_dim, int dtype, void* stream);
 
-/* kvb_append of keys that are turned on the way, and (q not NULL) queries turned beside it into q_out, in one launch.  Keys go from the turn into
+/* kvb_append of keys that are turned on the way, and (q not NULL) queries turned beside it into q_out.  Keys go from the turn into
  * the cache's own rotation in fp32, without the rounding to `dtype` that kvb_rope_rows followed by kvb_append makes.  q, q_out:
  * [tokens][q_heads][head_dim]; k, v: [tokens][kv_heads][head_dim]; strides in elements from token to token.  q_out may be q itself; it shares no
  * other memory with q, k, v or the positions.  Positions that are not contiguous set KVB_ERR_POSITIONS, and the call leaves cache and q_out alone. */
@@ -316,7 +316,8 @@ int kvb_linear_decode(const kvb_linear* layer, const void* q, int64_t q_stride, 
 
 /* The same over several tokens of each sequence, packed one sequence behind another: rows offsets_dev[b] .. offsets_dev[b + 1] - 1 belong to sequence
  * b (offsets_dev[batch + 1], not falling, within 0..tokens; a sequence without rows has its state copied).  Rows outside all sequences are left as they are.
- * Offsets that fall or leave the rows set KVB_ERR_POSITIONS; that sequence is left alone.  workspace: kvb_linear_workspace_bytes(tokens, batch, ...) bytes. */
+ * Offsets that fall or leave the rows set KVB_ERR_POSITIONS; that sequence is left alone.  workspace: kvb_linear_workspace_bytes(tokens, batch, ...) bytes, not shared by
+ * calls that overlap on the GPU. */
 size_t kvb_linear_workspace_bytes(int tokens, int batch, int v_heads, int head_dim);
 int kvb_linear_chunk(const kvb_linear* layer, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                      const int32_t* offsets_dev, int batch, int tokens, const int32_t* reads_dev, const int32_t* writes_dev, float scale, void* workspace, void* out,
