@@ -26,6 +26,17 @@ def _stream():
 
 
 # Checks of the calls whose rows may be parts of wider ones.  A step makes them in every layer: what is right is seen in a few comparisons.
+def stream_for(*tensors) -> int:
+    """The current stream, for a call on these tensors; one that is not on the current device is refused."""
+    device = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != device or device < 0:
+            raise ValueError(f"tensors of one CUDA device: got {', '.join(str(t.device) for t in tensors)}")
+    if device != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors of the current device, cuda:{torch._C._cuda_getDevice()}: got cuda:{device}")
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
 def row_stride(x: torch.Tensor, heads: int, head_dim: int, dtype: torch.dtype, tokens: int) -> int:
     """Elements from token to token of rows [tokens, heads, head_dim] whose heads are packed; anything else is refused."""
     if x.shape == (tokens, heads, head_dim) and x.dtype is dtype:
@@ -108,7 +119,8 @@ class KvarnLayer:
             qs = row_stride(q, qh, d, dtype, tokens)
             q_out = torch.empty_like(q) if q_out is None else q_out
             os = row_stride(q_out, qh, d, dtype, tokens)
-        capi.check(capi.load().kvb_rope_append(self.ref, rope.ref, _ptr(q), qs, _ptr(q_out), os, k.data_ptr(), ks, v.data_ptr(), vs, at, tokens, _stream()))
+        stream = stream_for(self.stage, rope.inv_freq, k, v, positions) if q is None else stream_for(self.stage, rope.inv_freq, k, v, positions, q, q_out)
+        capi.check(capi.load().kvb_rope_append(self.ref, rope.ref, _ptr(q), qs, _ptr(q_out), os, k.data_ptr(), ks, v.data_ptr(), vs, at, tokens, stream))
         return q_out
 
     # ---- rows back as keys and values (the reference: its bf16 mirror, kvarn128_window*)
@@ -121,7 +133,7 @@ class KvarnLayer:
         for x in (out_k, out_v):
             if x.shape != shape or x.dtype is not self.dtype or not x.is_contiguous():
                 raise ValueError(f"outputs: packed rows {list(shape)} of {self.dtype}")
-        capi.check(capi.load().kvb_read_rows(self.ref, begin, tokens, at, out_k.data_ptr(), out_v.data_ptr(), _stream()))
+        capi.check(capi.load().kvb_read_rows(self.ref, begin, tokens, at, out_k.data_ptr(), out_v.data_ptr(), stream_for(self.stage, pos, out_k, out_v)))
         return out_k, out_v
 
     # ---- kvarn128_decode_tile

@@ -7,7 +7,7 @@ import functools
 import torch
 
 from . import capi
-from .cache import _stream, check_indices, row_stride
+from .cache import check_indices, row_stride, stream_for
 
 
 @functools.lru_cache(maxsize=256)
@@ -31,7 +31,7 @@ class LinearAttention:
                                  head_dim=head_dim, dtype=capi.DTYPE_BF16 if dtype == torch.bfloat16 else capi.DTYPE_F16,
                                  error_word=self.error_word.data_ptr())
         self.ref = C.byref(self.c)
-        self._ws = None
+        self._ws = []
 
     def _device_key(self) -> int:
         return torch._C._cuda_getDevice() if self.device.type == "cuda" else -1
@@ -50,25 +50,26 @@ class LinearAttention:
         qs, ks, vs = row_stride(q, qk, d, dtype, batch), row_stride(k, qk, d, dtype, batch), row_stride(v, self.v_heads, d, dtype, batch)
         out = self._out(batch, v, out)
         capi.check(capi.load().kvb_linear_decode(self.ref, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, batch, check_indices(reads, batch, "reads"),
-                                                 check_indices(writes, batch, "writes"), scale, out.data_ptr(), _stream()))
+                                                 check_indices(writes, batch, "writes"), scale, out.data_ptr(), stream_for(self.state, q, k, v, reads, writes, out)))
         return out
 
     def workspace(self, tokens: int, batch: int) -> torch.Tensor:
-        """Scratch for chunk calls.  One buffer per layer that only ever grows: a CUDA graph that captured its address stays valid as long as the
-        first call (made before the capture) asked for the largest shape the graph uses."""
-        n = _workspace_bytes(self._device_key(), tokens, batch, self.v_heads, self.head_dim)
-        if self._ws is None or self._ws.numel() * 4 < n:
-            self._ws = torch.empty((n + 3) // 4, dtype=torch.float32, device=self.device)
-        return self._ws
+        """Scratch for chunk calls: the layer's own, which its calls share, so they do not overlap on the GPU.  Where a call wants more, the next buffer is
+        at least twice as large and the ones before stay as they are: a CUDA graph may have captured their addresses."""
+        n = (_workspace_bytes(self._device_key(), tokens, batch, self.v_heads, self.head_dim) + 3) // 4
+        if not self._ws or self._ws[-1].numel() < n:
+            self._ws.append(torch.empty(max(n, 2 * self._ws[-1].numel()) if self._ws else n, dtype=torch.float32, device=self.device))
+        return self._ws[-1]
 
     def chunk(self, q, k, v, offsets: torch.Tensor, scale: float, reads: torch.Tensor, writes: torch.Tensor, out=None) -> torch.Tensor:
         """Several tokens of each sequence, packed: rows offsets[b] .. offsets[b + 1] - 1 are sequence b's; offsets: int32 [batch + 1] on the device."""
         tokens, qk, d, dtype, batch = q.shape[0], self.qk_heads, self.head_dim, self.dtype, reads.shape[0]
         qs, ks, vs = row_stride(q, qk, d, dtype, tokens), row_stride(k, qk, d, dtype, tokens), row_stride(v, self.v_heads, d, dtype, tokens)
         out = self._out(tokens, v, out)
+        stream = stream_for(self.state, q, k, v, offsets, reads, writes, out)
         capi.check(capi.load().kvb_linear_chunk(self.ref, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, check_indices(offsets, batch + 1, "offsets"),
                                                 batch, tokens, check_indices(reads, batch, "reads"), check_indices(writes, batch, "writes"), scale,
-                                                self.workspace(tokens, batch).data_ptr(), out.data_ptr(), _stream()))
+                                                self.workspace(tokens, batch).data_ptr(), out.data_ptr(), stream))
         return out
 
     def errors(self) -> int:

@@ -7,7 +7,7 @@ import ctypes as C
 import torch
 
 from . import capi
-from .cache import _stream, check_indices, row_stride
+from .cache import check_indices, row_stride, stream_for
 
 _SCALINGS = {"none": capi.ROPE_PLAIN, "linear": capi.ROPE_LINEAR, "ntk": capi.ROPE_NTK, "yarn": capi.ROPE_YARN}
 _DTYPES = {torch.float16: capi.DTYPE_F16, torch.bfloat16: capi.DTYPE_BF16}
@@ -38,5 +38,5 @@ class Rope:
         stride = row_stride(x, heads, dim, x.dtype, tokens)
         out = torch.empty_like(x) if out is None else out
         capi.check(capi.load().kvb_rope_rows(self.ref, x.data_ptr(), stride, out.data_ptr(), row_stride(out, heads, dim, x.dtype, tokens), at, tokens, heads,
-                                             dim, dtype, _stream()))
+                                             dim, dtype, stream_for(self.inv_freq, x, positions, out)))
         return out

@@ -439,3 +439,27 @@ def test_same_inputs_same_bits():
     for _ in range(5):
         layer.state.copy_(first)
         assert torch.equal(layer.chunk(*args), out) and torch.equal(layer.state, state)
+
+
+def test_a_captured_call_keeps_its_workspace():
+    """A later call that needs a larger workspace, and allocations after it, do not touch what a graph has captured."""
+    import torch
+
+    vh, D, few, many = 2, 128, 700, 9000
+    layer = _layer(1, vh, D, 2, "bf16")
+    first = _fill(layer, 4)
+    q, k, v = _inputs(1, vh, D, many, "bf16", 8)
+    r, w = _i32([0]), _i32([1])
+    args = (q[:few], k[:few], v[:few], _i32([0, few]), 0.1, r, w)
+    want, state = layer.chunk(*args).clone(), layer.state.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer.chunk(*args)
+    size = layer.workspace(few, 1).numel()
+    layer.chunk(q, k, v, _i32([0, many]), 0.1, r, w)
+    assert layer.workspace(many, 1).numel() > size
+    others = [torch.full((size,), 3.0, dtype=torch.float32, device="cuda") for _ in range(8)]
+    layer.state.copy_(first)
+    graph.replay()
+    assert torch.equal(out, want) and torch.equal(layer.state, state) and layer.errors() == 0
+    assert all(bool((x == 3.0).all()) for x in others)

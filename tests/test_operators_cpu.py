@@ -175,3 +175,26 @@ def test_python_refuses_rows_that_are_not_rows():
     for bad in ((at, 7), (at.long(), 8), (at[::2], 4), (at.view(2, 4), 8)):
         with pytest.raises(ValueError):
             check_indices(*bad, "x")
+
+
+def test_tensors_off_the_device_are_refused():
+    """Rows, indices and layers in host memory: a ValueError before the library sees an address."""
+    import torch
+
+    p = pkg()
+    rope = p.Rope(64, device="cpu")
+    x, at = torch.zeros(2, 4, 128, dtype=torch.float16), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="device"):
+        rope.rows(x, at)
+    layer = p.KvarnLayer(128, 4, 8, 4, torch.arange(4, dtype=torch.int32), device="cpu")
+    with pytest.raises(ValueError, match="device"):
+        layer.rope_append(rope, x, x, at)
+    with pytest.raises(ValueError, match="device"):
+        layer.rope_append(rope, x, x, at, q=torch.zeros(2, 8, 128, dtype=torch.float16))
+    with pytest.raises(ValueError, match="device"):
+        layer.read_rows(0, 2, at[:1])
+    mix = p.LinearAttention(4, 4, 128, torch.zeros(4), 2, dtype=torch.float16, device="cpu")
+    with pytest.raises(ValueError, match="device"):
+        mix.decode(x, x, x, 1.0, at, at)
+    with pytest.raises(ValueError, match="device"):
+        mix.chunk(x, x, x, torch.zeros(3, dtype=torch.int32), 1.0, at, at)
