@@ -26,15 +26,17 @@ def _stream():
 
 
 # Checks of the calls whose rows may be parts of wider ones.  A step makes them in every layer: what is right is seen in a few comparisons.
-def stream_for(*tensors) -> int:
-    """The current stream, for a call on these tensors; one that is not on the current device is refused."""
-    device = tensors[0].get_device()
+def stream_for(device: int, *tensors) -> int:
+    """The current stream, for a call of a layer on `device` with these tensors; where one is not on the current device the call is refused."""
     for t in tensors:
         if t.get_device() != device or device < 0:
-            raise ValueError(f"tensors of one CUDA device: got {', '.join(str(t.device) for t in tensors)}")
-    if device != torch._C._cuda_getDevice():
-        raise ValueError(f"tensors of the current device, cuda:{torch._C._cuda_getDevice()}: got cuda:{device}")
-    return torch._C._cuda_getCurrentRawStream(device)
+            raise ValueError(f"tensors of the layer's CUDA device (index {device}): got {', '.join(str(t.device) for t in tensors)}")
+    if device != _current_device():
+        raise ValueError(f"tensors of the current device, cuda:{_current_device()}: got cuda:{device}")
+    return _raw_stream(device)
+
+
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def row_stride(x: torch.Tensor, heads: int, head_dim: int, dtype: torch.dtype, tokens: int) -> int:
@@ -96,6 +98,7 @@ class KvarnLayer:
             dtype=capi.DTYPE_BF16 if dtype == torch.bfloat16 else capi.DTYPE_F16, sinkhorn_iters=sinkhorn_iters,
             error_word=self.error_word.data_ptr())
         self.ref = C.byref(self.c)
+        self.index = self.stage.get_device()
         self._ws = None
         self._pws = None
 
@@ -119,7 +122,9 @@ class KvarnLayer:
             qs = row_stride(q, qh, d, dtype, tokens)
             q_out = torch.empty_like(q) if q_out is None else q_out
             os = row_stride(q_out, qh, d, dtype, tokens)
-        stream = stream_for(self.stage, rope.inv_freq, k, v, positions) if q is None else stream_for(self.stage, rope.inv_freq, k, v, positions, q, q_out)
+        stream = stream_for(self.index, k, v, positions) if q is None else stream_for(self.index, k, v, positions, q, q_out)
+        if rope.index != self.index:
+            raise ValueError(f"rope on device {rope.index}, the layer on {self.index}")
         capi.check(capi.load().kvb_rope_append(self.ref, rope.ref, _ptr(q), qs, _ptr(q_out), os, k.data_ptr(), ks, v.data_ptr(), vs, at, tokens, stream))
         return q_out
 
@@ -133,7 +138,7 @@ class KvarnLayer:
         for x in (out_k, out_v):
             if x.shape != shape or x.dtype is not self.dtype or not x.is_contiguous():
                 raise ValueError(f"outputs: packed rows {list(shape)} of {self.dtype}")
-        capi.check(capi.load().kvb_read_rows(self.ref, begin, tokens, at, out_k.data_ptr(), out_v.data_ptr(), stream_for(self.stage, pos, out_k, out_v)))
+        capi.check(capi.load().kvb_read_rows(self.ref, begin, tokens, at, out_k.data_ptr(), out_v.data_ptr(), stream_for(self.index, pos, out_k, out_v)))
         return out_k, out_v
 
     # ---- kvarn128_decode_tile

@@ -31,6 +31,7 @@ class LinearAttention:
                                  head_dim=head_dim, dtype=capi.DTYPE_BF16 if dtype == torch.bfloat16 else capi.DTYPE_F16,
                                  error_word=self.error_word.data_ptr())
         self.ref = C.byref(self.c)
+        self.index = self.state.get_device()
         self._ws = []
 
     def _device_key(self) -> int:
@@ -50,7 +51,7 @@ class LinearAttention:
         qs, ks, vs = row_stride(q, qk, d, dtype, batch), row_stride(k, qk, d, dtype, batch), row_stride(v, self.v_heads, d, dtype, batch)
         out = self._out(batch, v, out)
         capi.check(capi.load().kvb_linear_decode(self.ref, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, batch, check_indices(reads, batch, "reads"),
-                                                 check_indices(writes, batch, "writes"), scale, out.data_ptr(), stream_for(self.state, q, k, v, reads, writes, out)))
+                                                 check_indices(writes, batch, "writes"), scale, out.data_ptr(), stream_for(self.index, q, k, v, reads, writes, out)))
         return out
 
     def workspace(self, tokens: int, batch: int) -> torch.Tensor:
@@ -66,7 +67,7 @@ class LinearAttention:
         tokens, qk, d, dtype, batch = q.shape[0], self.qk_heads, self.head_dim, self.dtype, reads.shape[0]
         qs, ks, vs = row_stride(q, qk, d, dtype, tokens), row_stride(k, qk, d, dtype, tokens), row_stride(v, self.v_heads, d, dtype, tokens)
         out = self._out(tokens, v, out)
-        stream = stream_for(self.state, q, k, v, offsets, reads, writes, out)
+        stream = stream_for(self.index, q, k, v, offsets, reads, writes, out)
         capi.check(capi.load().kvb_linear_chunk(self.ref, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, check_indices(offsets, batch + 1, "offsets"),
                                                 batch, tokens, check_indices(reads, batch, "reads"), check_indices(writes, batch, "writes"), scale,
                                                 self.workspace(tokens, batch).data_ptr(), out.data_ptr(), stream))

@@ -27,6 +27,7 @@ class Rope:
         self.inv_freq = torch.tensor(list(host), dtype=torch.float64).to(device)
         self.c = capi.kvb_rope(inv_freq=self.inv_freq.data_ptr(), factor=self.factor, rotary_dim=rotary_dim, interleaved=int(interleaved))
         self.ref = C.byref(self.c)
+        self.index = self.inv_freq.get_device()
 
     def rows(self, x: torch.Tensor, positions: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """x: [tokens, heads, head_dim] (fp16 or bf16), packed or part of wider rows; positions: int32 [tokens] on the device.  `out` may be x."""
@@ -38,5 +39,5 @@ class Rope:
         stride = row_stride(x, heads, dim, x.dtype, tokens)
         out = torch.empty_like(x) if out is None else out
         capi.check(capi.load().kvb_rope_rows(self.ref, x.data_ptr(), stride, out.data_ptr(), row_stride(out, heads, dim, x.dtype, tokens), at, tokens, heads,
-                                             dim, dtype, stream_for(self.inv_freq, x, positions, out)))
+                                             dim, dtype, stream_for(self.index, x, positions, out)))
         return out
