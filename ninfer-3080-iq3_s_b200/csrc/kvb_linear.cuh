@@ -42,10 +42,10 @@ struct LinearView {
         bool shared = false;
         for (int i = threadIdx.x; i < batch; i += blockDim.x)
             if (i != seq) shared = shared || writes[i] == s.to || reads[i] == s.to || writes[i] == s.from;
-        s.valid = judge(s, __syncthreads_or(shared) != 0);
+        s.valid = allowed(s, __syncthreads_or(shared) != 0);
         return s;
     }
-    __device__ __forceinline__ bool judge(const Sequence& s, bool shared) const {
+    __device__ __forceinline__ bool allowed(const Sequence& s, bool shared) const {
         const bool rows = s.begin >= 0 && s.end >= s.begin && s.end <= tokens;
         const bool pool = s.from >= 0 && s.from < slots && s.to >= 0 && s.to < slots;
         if (!rows) flag(KVB_ERR_POSITIONS);

@@ -148,7 +148,7 @@ __device__ __forceinline__ Unit unit_of(const ChunkCall& P, int unit, int head, 
     u.seq.to = writes[seq];
     const bool other = tid < V.batch && tid != seq;
     const bool shared = __syncthreads_or(other && (writes[tid] == u.seq.to || reads[tid] == u.seq.to || writes[tid] == u.seq.from)) != 0;
-    u.seq.valid = u.count > 0 && V.judge(u.seq, shared);
+    u.seq.valid = u.count > 0 && V.allowed(u.seq, shared);
     return u;
 }
 
