@@ -316,8 +316,9 @@ int kvb_linear_decode(const kvb_linear* layer, const void* q, int64_t q_stride, 
 
 /* The same over several tokens of each sequence, packed one sequence behind another: rows offsets_dev[b] .. offsets_dev[b + 1] - 1 belong to sequence
  * b (offsets_dev[batch + 1], not falling, within 0..tokens; a sequence without rows has its state copied).  Rows outside all sequences are left as they are.
- * Offsets that fall or leave the rows set KVB_ERR_POSITIONS; that sequence is left alone.  workspace: kvb_linear_workspace_bytes(tokens, batch, ...) bytes, not shared by
- * calls that overlap on the GPU. */
+ * Offsets that fall or leave the rows set KVB_ERR_POSITIONS; that sequence is left alone.  Where offsets that fall make sequences share rows, an output is
+ * that of one of them, and a sequence may be left alone for want of places in the workspace (KVB_ERR_POSITIONS).
+ * workspace: kvb_linear_workspace_bytes(tokens, batch, ...) bytes, not shared by calls that overlap on the GPU. */
 size_t kvb_linear_workspace_bytes(int tokens, int batch, int v_heads, int head_dim);
 int kvb_linear_chunk(const kvb_linear* layer, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                      const int32_t* offsets_dev, int batch, int tokens, const int32_t* reads_dev, const int32_t* writes_dev, float scale, void* workspace, void* out,

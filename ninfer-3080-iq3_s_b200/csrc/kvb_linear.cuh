@@ -2,13 +2,11 @@
 #pragma once
 
 #include "kvb_common.cuh"
+#include "kvb_linear_plan.hpp"
 #include "kvb_ptx.cuh"
 #include "kvb_rope.cuh"
 
 namespace kvb {
-
-constexpr int kMostSequences = 256;  // of one call
-constexpr int kLinearChunk = 64;     // tokens that the chunked form takes at a time
 
 // Rows [begin, end) of one sequence and the slots its state is read from and written to.
 struct Sequence {
@@ -60,9 +58,8 @@ struct LinearView {
     }
 };
 
-// The chunked form: tokens of a segment (a multiple of a chunk), the grid's units (segments of all sequences, at most), and the launches.
-int linear_segment(int tokens, int batch, int v_heads);
-int linear_units(int tokens, int batch, int segment);
+// The chunked form: tokens of a segment on this device, and the launches.
+inline int linear_segment(int tokens, int batch, int v_heads) { return linear_segment_of(tokens, batch, v_heads, device_sm_count()); }
 int linear_chunks(const LinearView& V, bool bf16, bool aligned, void* workspace, cudaStream_t stream);
 
 int check_linear(const kvb_linear* layer, const char* who);

@@ -103,26 +103,14 @@ __device__ __forceinline__ Unit unit_of(const ChunkCall& P, int unit, int head, 
         writes[tid] = V.writes[tid];
     }
     __syncthreads();
-    if (tid < V.batch) {
-        const int64_t mine = static_cast<int64_t>(offsets[tid + 1]) - offsets[tid];
-        int rank = 0;
-        for (int s = 0; s < V.batch; ++s) {
-            const int64_t length = static_cast<int64_t>(offsets[s + 1]) - offsets[s];
-            rank += length > mine || (length == mine && s < tid);
-        }
-        order[rank] = tid;
-    }
+    if (tid < V.batch) order[linear_rank(offsets, tid, V.batch)] = tid;
     __syncthreads();
     if (tid < 32) {
         int base = 0;
         bool any = false;
         for (int s0 = 0; s0 < V.batch; s0 += 32) {
             const int seq = s0 + lane < V.batch ? order[s0 + lane] : V.batch;
-            int count = 0;
-            if (seq < V.batch) {
-                const int64_t length = static_cast<int64_t>(offsets[seq + 1]) - offsets[seq];
-                count = length <= 0 || length > V.tokens ? 1 : static_cast<int>((length + P.segment - 1) / P.segment);
-            }
+            const int count = seq < V.batch ? linear_segments(offsets, seq, V.tokens, P.segment) : 0;
             int sum = count;  // inclusive
 #pragma unroll
             for (int step = 1; step < 32; step <<= 1) {
@@ -135,7 +123,7 @@ __device__ __forceinline__ Unit unit_of(const ChunkCall& P, int unit, int head, 
             base += __shfl_sync(0xffffffffu, sum, 31);
         }
         if (!any && lane == 0) found[0] = found[1] = found[2] = 0;
-        // sequences that overlap have more segments than the grid has units: what is left out is reported
+        // sequences that share rows have more segments than the grid has units: the ones left alone for it are reported
         if (unit == 0 && base > static_cast<int>(gridDim.y)) V.flag(KVB_ERR_POSITIONS);
     }
     __syncthreads();
@@ -148,7 +136,7 @@ __device__ __forceinline__ Unit unit_of(const ChunkCall& P, int unit, int head, 
     u.seq.to = writes[seq];
     const bool other = tid < V.batch && tid != seq;
     const bool shared = __syncthreads_or(other && (writes[tid] == u.seq.to || reads[tid] == u.seq.to || writes[tid] == u.seq.from)) != 0;
-    u.seq.valid = u.count > 0 && V.allowed(u.seq, shared);
+    u.seq.valid = u.count > 0 && V.allowed(u.seq, shared) && linear_fits(unit, u.index, u.count, static_cast<int>(gridDim.y));
     return u;
 }
 
@@ -750,25 +738,6 @@ template <int D, bool kBf16> int launch_chunks(const ChunkCall& P, int units, cu
 }
 
 }  // namespace
-
-// Segments of a sequence of the average length: what costs least, in chunks of the second launch, by waves of CTAs (one an SM).  A CTA costs 4
-// chunks beside its own there (states in and out, the pipeline's start), the first launch 0.45 of a chunk and 2.5.  Measured on B200, 32 value heads of 128
-// dims: 2.1 us a chunk in the second launch, 0.9 in the first.
-int linear_segment(int tokens, int batch, int v_heads) {
-    const int64_t sequences = batch < 1 ? 1 : batch, units = sequences * v_heads, sms = device_sm_count();
-    const int64_t length = (static_cast<int64_t>(tokens) + sequences * kC - 1) / (sequences * kC);
-    const int64_t whole = (static_cast<int64_t>(tokens) + kC - 1) / kC;  // one segment, whichever sequence has the tokens
-    auto waves = [&](int64_t ctas) { return static_cast<double>((ctas + sms - 1) / sms); };
-    double least = waves(units) * (static_cast<double>(length) + 4.0);
-    int64_t segment = whole;
-    for (int64_t n = 2; n <= length && n <= 64; ++n) {
-        const int64_t chunks = (length + n - 1) / n;
-        const double cost = waves(units * n) * (static_cast<double>(chunks) + 4.0) + waves(units * (n - 1)) * (0.45 * static_cast<double>(chunks) + 2.5);
-        if (cost < least) least = cost, segment = chunks;
-    }
-    return static_cast<int>((segment < 1 ? 1 : segment) * kC);
-}
-int linear_units(int tokens, int batch, int segment) { return tokens / segment + batch; }
 
 namespace {
 
