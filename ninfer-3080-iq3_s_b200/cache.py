@@ -25,6 +25,16 @@ def _stream():
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
+_DTYPE_CODES = {torch.float16: capi.DTYPE_F16, torch.bfloat16: capi.DTYPE_BF16}
+
+
+def dtype_code(dtype: torch.dtype) -> int:
+    """The library's number for the type of a layer's rows; a type it does not compute in is refused."""
+    if dtype not in _DTYPE_CODES:
+        raise ValueError(f"dtype: float16 or bfloat16, got {dtype}")
+    return _DTYPE_CODES[dtype]
+
+
 # Checks of the calls whose rows may be parts of wider ones.  A step makes them in every layer: what is right is seen in a few comparisons.
 def stream_for(device: int, *tensors) -> int:
     """The current stream, for a call of a layer on `device` with these tensors; where one is not on the current device the call is refused."""
@@ -75,7 +85,7 @@ class KvarnLayer:
 
     def __init__(self, head_dim: int, kv_heads: int, q_heads: int, pages: int, table: torch.Tensor,
                  dtype: torch.dtype = torch.float16, sinkhorn_iters: int = 0, device: str = "cuda"):
-        lib = capi.load()
+        lib, code = capi.load(), dtype_code(dtype)
         self.head_dim, self.kv_heads, self.q_heads, self.pages = head_dim, kv_heads, q_heads, pages
         self.dtype = dtype
         self.device = torch.device(device)
@@ -95,7 +105,7 @@ class KvarnLayer:
             v_scale=self.v_scale.data_ptr(), stage=self.stage.data_ptr(), table_direct=self.table.data_ptr(),
             tables=None, table_rows=None, table_stride=0, table_len=self.table.numel(), pages=pages,
             kv_heads=kv_heads, q_heads=q_heads, head_dim=head_dim,
-            dtype=capi.DTYPE_BF16 if dtype == torch.bfloat16 else capi.DTYPE_F16, sinkhorn_iters=sinkhorn_iters,
+            dtype=code, sinkhorn_iters=sinkhorn_iters,
             error_word=self.error_word.data_ptr())
         self.ref = C.byref(self.c)
         self.index = self.stage.get_device()
@@ -240,7 +250,7 @@ class DecodeBatch:
         first = layers[0]
         assert all((L.head_dim, L.kv_heads, L.q_heads, L.dtype) == (first.head_dim, first.kv_heads, first.q_heads, first.dtype) for L in layers)
         self.layers, self.n = list(layers), len(layers)
-        self.geo = (first.kv_heads, first.q_heads, first.head_dim, capi.DTYPE_BF16 if first.dtype == torch.bfloat16 else capi.DTYPE_F16)
+        self.geo = (first.kv_heads, first.q_heads, first.head_dim, dtype_code(first.dtype))
         raw = b"".join(bytes(L.c) for L in layers)
         self.descriptors = torch.frombuffer(bytearray(raw), dtype=torch.uint8).to(first.device)
         self.bounds = (C.c_int32 * self.n)(*[int(x) for x in kv_len_max])

@@ -7,7 +7,7 @@ import functools
 import torch
 
 from . import capi
-from .cache import check_indices, row_stride, stream_for
+from .cache import check_indices, dtype_code, row_stride, stream_for
 
 
 @functools.lru_cache(maxsize=256)
@@ -22,14 +22,14 @@ class LinearAttention:
                  device: str = "cuda"):
         if tuple(log_decay.shape) != (v_heads,):
             raise ValueError(f"log_decay: [{v_heads}], got {tuple(log_decay.shape)}")
+        code = dtype_code(dtype)
         self.qk_heads, self.v_heads, self.head_dim, self.slots, self.dtype = qk_heads, v_heads, head_dim, slots, dtype
         self.device = torch.device(device)
         self.state = torch.zeros((slots, v_heads, head_dim, head_dim), dtype=torch.float32, device=self.device)
         self.log_decay = log_decay.to(device=self.device, dtype=torch.float32).contiguous()
         self.error_word = torch.zeros(1, dtype=torch.int32, device=self.device)
         self.c = capi.kvb_linear(state=self.state.data_ptr(), log_decay=self.log_decay.data_ptr(), slots=slots, qk_heads=qk_heads, v_heads=v_heads,
-                                 head_dim=head_dim, dtype=capi.DTYPE_BF16 if dtype == torch.bfloat16 else capi.DTYPE_F16,
-                                 error_word=self.error_word.data_ptr())
+                                 head_dim=head_dim, dtype=code, error_word=self.error_word.data_ptr())
         self.ref = C.byref(self.c)
         self.index = self.state.get_device()
         self._ws = []

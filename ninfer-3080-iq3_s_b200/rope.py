@@ -7,10 +7,9 @@ import ctypes as C
 import torch
 
 from . import capi
-from .cache import check_indices, row_stride, stream_for
+from .cache import _DTYPE_CODES, check_indices, row_stride, stream_for
 
 _SCALINGS = {"none": capi.ROPE_PLAIN, "linear": capi.ROPE_LINEAR, "ntk": capi.ROPE_NTK, "yarn": capi.ROPE_YARN}
-_DTYPES = {torch.float16: capi.DTYPE_F16, torch.bfloat16: capi.DTYPE_BF16}
 
 
 class Rope:
@@ -31,7 +30,7 @@ class Rope:
 
     def rows(self, x: torch.Tensor, positions: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """x: [tokens, heads, head_dim] (fp16 or bf16), packed or part of wider rows; positions: int32 [tokens] on the device.  `out` may be x."""
-        dtype = _DTYPES.get(x.dtype)
+        dtype = _DTYPE_CODES.get(x.dtype)
         if dtype is None or x.dim() != 3:
             raise ValueError(f"x: rows [tokens, heads, head_dim] of float16 or bfloat16, got {tuple(x.shape)} of {x.dtype}")
         tokens, heads, dim = x.shape
