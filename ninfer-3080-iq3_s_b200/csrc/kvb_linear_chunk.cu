@@ -45,7 +45,7 @@ namespace kvb {
 namespace {
 
 constexpr int kC = kLinearChunk;  // tokens of a chunk
-constexpr int kStages = 3;
+constexpr int kStages = kLinearStages;
 constexpr int kStateWarps = 8, kRowWarps = 8;
 // the last eight: warps 0, 1, 4, 5 of them P (rows 0 .. 63 of tensor memory are a warp's by its number mod 4)
 constexpr int kLastWarps = kStateWarps + kRowWarps, kStateMmaWarp = kLastWarps + 2, kLoadWarp = kLastWarps + 3, kRowMmaWarp = kLastWarps + 6, kStoreWarp = kLastWarps + 7;
@@ -71,6 +71,7 @@ template <int D> struct LinearSmem {
     uint64_t full[kStages], done[kStages], rows_done[kStages], scores[kStages], state_ready[3], p_ready[2], keys_ready[2], out_read[2], out_ready[2], out_free[2], most_ready[2], loaded, drained[2];
     uint32_t tmem_base;
     int abort_flag;
+    int issued;  // chunks whose tiles were asked for by TMA
     int unit[3];
 };
 
@@ -268,6 +269,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
         mbar_init(&sm.drained[1], 1);
         mbar_fence_init();
         sm.abort_flag = 0;
+        sm.issued = 0;
     }
     if (threadIdx.x < 4 * kC) {
         const int copy = threadIdx.x / (2 * kC), x = threadIdx.x % (2 * kC), n = kC - 1 - x - copy;
@@ -349,6 +351,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                     load_tile<D>(st.k, P.k, qk_head, t, &sm.full[stage]);
                     if (!kSums) load_tile<D>(st.q, P.q, qk_head, t, &sm.full[stage]);
                     load_tile<D>(st.v, P.v, head, t, &sm.full[stage]);
+                    sm.issued = c + 1;
                 }
             } else {
                 const int valid = min(kC, end - static_cast<int>(t));
@@ -361,9 +364,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
             }
             __syncwarp();
         }
-        // no copy lands in shared memory that is no longer this CTA's
-        if (failed && P.aligned)
-            for (int c = max(0, chunks - kStages); c < chunks; ++c) mbar_wait_bounded(&sm.full[c % kStages], (c / kStages) & 1);
     } else if (warp == kStoreWarp) {
         // ---- stores
         const bool wide = (reinterpret_cast<uintptr_t>(V.out) & 15u) == 0;
@@ -457,12 +457,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                     __syncwarp();
                 }
             }
-        }
-        if (failed) {  // nothing is freed under MMAs that still run
-            uint64_t* const drained = &sm.drained[warp == kRowMmaWarp];
-            if (tc::elect_one()) tc::commit(drained);
-            __syncwarp();
-            mbar_wait_bounded(drained, 0);
         }
     } else if (warp < kKeyWarps) {
         // ---- state warps: rows 32 (warp % 4) + lane of S^T, columns by warp / 4
@@ -716,7 +710,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
     }
     if (failed && lane == 0 && V.error_word != nullptr) atomicOr(V.error_word, KVB_ERR_WAIT_TIMEOUT);
     tc::fence_before_sync();
-    __syncthreads();
+    // Where any warp gave up, others may have gone through: no copy lands in shared memory, and no MMA runs on tensor memory, that is no longer this CTA's.
+    if (__syncthreads_or(failed)) {
+        if (warp == kLoadWarp) {
+            const int issued = sm.issued;
+            for (int c = linear_first_in_flight(issued); c < issued; ++c) mbar_wait_bounded(&sm.full[c % kStages], (c / kStages) & 1);
+        } else if (warp == kStateMmaWarp || warp == kRowMmaWarp) {
+            uint64_t* const drained = &sm.drained[warp == kRowMmaWarp];
+            if (tc::elect_one()) tc::commit(drained);
+            __syncwarp();
+            mbar_wait_bounded(drained, 0);
+        }
+        tc::fence_before_sync();
+        __syncthreads();
+    }
     if (warp == kStateMmaWarp) {
         tc::fence_after_sync();
         tc::tmem_dealloc(tmem, kTmemCols);

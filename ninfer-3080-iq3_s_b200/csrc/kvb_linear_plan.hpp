@@ -56,4 +56,9 @@ KVB_LINEAR_PLAN int linear_rank(const int32_t* offsets, int seq, int batch) {
 // left alone, by all of its units and in both launches.
 KVB_LINEAR_PLAN bool linear_fits(int unit, int index, int count, int units) { return unit - index + count <= units; }
 
+// Tiles come chunk by chunk into kLinearStages stages in turn, a stage's next one when the chunk before it there is done with.  Of `issued` chunks that were asked
+// for, the first that may still be under way; chunk c's barrier is that of its stage, in phase c / kLinearStages.
+constexpr int kLinearStages = 3;
+KVB_LINEAR_PLAN int linear_first_in_flight(int issued) { return issued > kLinearStages ? issued - kLinearStages : 0; }
+
 }  // namespace kvb
