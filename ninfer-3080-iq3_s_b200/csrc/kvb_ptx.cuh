@@ -60,8 +60,8 @@ constexpr bool kStepWaitsK = (KVB_STEP_PROBES_K) > 0, kStepWaitsV = (KVB_STEP_PR
 
 // The same wait for lanes that may have diverged (some found the barrier complete at their first probe): no vote.
 // Every lane probes the same barrier phase, so a lane can run out of probes only if no lane ever saw it complete.
-__device__ __forceinline__ bool mbar_wait_lane_bounded(uint64_t* bar, uint32_t parity) {
-    for (uint32_t i = 0; i < kSpinLimit; ++i)
+__device__ __forceinline__ bool mbar_wait_lane_bounded(uint64_t* bar, uint32_t parity, uint32_t probes = kSpinLimit) {
+    for (uint32_t i = 0; i < probes; ++i)
         if (mbar_try_wait(bar, parity)) return true;
     return false;
 }

@@ -23,6 +23,11 @@
 namespace kvb {
 namespace {
 
+// Probes of the wait for a CTA's n-th tile.  (A test builds the kernel with waits that give up at once while tiles are on their way.)
+#ifndef KVB_READ_PROBES
+#define KVB_READ_PROBES kSpinLimit
+#endif
+
 constexpr int kReadThreads = 128, kReadWarps = kReadThreads / 32;
 
 constexpr int kDimStride = 36;  // of a lane number's 32 dims: four lanes' 8 (16) bytes lie in different banks
@@ -162,9 +167,14 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(LayerView L, int beg
     for (int tile = first_tile; tile <= last_tile; tile += step, ++n) {
         const int buffer = n & 1;
         if (tid == 0) ask(tile + step, buffer ^ 1);
-        const bool ok = mbar_wait_lane_bounded(&sm.full[buffer], (n >> 1) & 1);
+        const bool ok = mbar_wait_lane_bounded(&sm.full[buffer], (n >> 1) & 1, KVB_READ_PROBES);
         if (__syncthreads_or(!ok)) {
-            if (tid == 0) L.flag(KVB_ERR_WAIT_TIMEOUT);
+            if (tid == 0) {
+                L.flag(KVB_ERR_WAIT_TIMEOUT);
+                // no copy lands in shared memory that is no longer this CTA's
+                mbar_wait_lane_bounded(&sm.full[buffer], (n >> 1) & 1);
+                if (tile + step <= last_tile) mbar_wait_lane_bounded(&sm.full[buffer ^ 1], ((n + 1) >> 1) & 1);
+            }
             return;
         }
         const int kind = sm.kind[buffer];
