@@ -318,6 +318,7 @@ int kvb_linear_decode(const kvb_linear* layer, const void* q, int64_t q_stride, 
  * b (offsets_dev[batch + 1], not falling, within 0..tokens; a sequence without rows has its state copied).  Rows outside all sequences are left as they are.
  * Offsets that fall or leave the rows set KVB_ERR_POSITIONS; that sequence is left alone.  Where offsets that fall make sequences share rows, an output is
  * that of one of them, and a sequence may be left alone for want of places in the workspace (KVB_ERR_POSITIONS).
+ * An infinite key leaves the recurrence's infinities; an infinite value may leave NaN in its column of the state, as may a decay that rounds to 0 on the way.
  * workspace: kvb_linear_workspace_bytes(tokens, batch, ...) bytes, not shared by calls that overlap on the GPU. */
 size_t kvb_linear_workspace_bytes(int tokens, int batch, int v_heads, int head_dim);
 int kvb_linear_chunk(const kvb_linear* layer, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,

@@ -165,6 +165,16 @@ template <bool kBf16> __device__ __forceinline__ uint32_t pack_pair(F2 x) {
     return pack_pair<kBf16>(f.x, f.y);
 }
 __device__ __forceinline__ F2 pair_of_words(uint32_t a, uint32_t b) { return F2(__uint_as_float(a), __uint_as_float(b)); }
+// What an infinite key leaves out of its first number is inf - inf: the first number alone has the key then.
+template <bool kBf16> __device__ __forceinline__ uint32_t zero_if_nan(uint32_t w) {
+    if constexpr (kBf16) {
+        const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&w);
+        return w & __heq2_mask(x, x);
+    } else {
+        const __half2 x = *reinterpret_cast<const __half2*>(&w);
+        return w & __heq2_mask(x, x);
+    }
+}
 // Instruction descriptor of 16-bit operands of either type (format 0 = f16, 1 = bf16).
 template <bool kBf16> __host__ __device__ constexpr uint32_t idesc_16(int m, int n, bool a_mn, bool b_mn) {
     return tc::idesc_f16(m, n, a_mn, b_mn) | (kBf16 ? (1u << 7) | (1u << 10) : 0u);
@@ -488,14 +498,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                     for (int e = 0; e < 4; ++e) {
                         const __nv_bfloat162 k = *reinterpret_cast<const __nv_bfloat162*>(&in[e]), x = __hmul2(k, w1), y = __hfma2(k, w2, __hfma2(k, w1, __hneg2(x)));
                         a[e] = *reinterpret_cast<const uint32_t*>(&x);
-                        b[e] = *reinterpret_cast<const uint32_t*>(&y);
+                        b[e] = zero_if_nan<kBf16>(*reinterpret_cast<const uint32_t*>(&y));
                     }
                 } else {  // small weights have too few bits in fp16
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const F2 x = mul2(pair_of<kBf16>(in[e]), F2(w, w));
                         a[e] = pack_pair<kBf16>(x);
-                        b[e] = pack_pair<kBf16>(sub2(x, pair_of<kBf16>(a[e])));
+                        b[e] = zero_if_nan<kBf16>(pack_pair<kBf16>(sub2(x, pair_of<kBf16>(a[e]))));
                     }
                 }
                 *reinterpret_cast<uint4*>(keys + 16 * u) = make_uint4(a[0], a[1], a[2], a[3]);
