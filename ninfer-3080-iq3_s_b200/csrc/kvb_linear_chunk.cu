@@ -9,8 +9,8 @@
 // Everything but the scores is computed transposed, head dims of v along the M rows of the MMAs: S^T stays in tensor memory as an fp32 accumulator from
 // chunk to chunk, and is an A operand there too; only rows of tokens as they come from global memory, decayed keys and P lie in shared memory.
 // Roundings: P, and the state as an operand, to the type, like the output that they are summed up to (both together as much as the output's own
-// rounding); decayed keys as two numbers of the type, whose sum has 16 bits of bf16 or 22 of fp16, so that states keep their precision over long
-// prompts: 3e-6 of the state's norm in bf16 (a third number would take 32 KB of shared memory that are not there).  Heads of 64 dims fill both halves
+// rounding); decayed keys as two numbers of the type, whose sum has 16 bits of bf16 or 22 of fp16 (2^-36 where these are less), so that states keep their
+// precision over long prompts: 4e-6 of the state's norm in bf16 (a third number would take 32 KB of shared memory that are not there), 2e-7 in fp16.  Heads of 64 dims fill both halves
 // of the M rows with the same 64; the scores' 64 rows are the first of 128, and what the others multiply is not looked at.
 //
 // Warps by role, so that a chunk's steps run beside its neighbours':
@@ -186,6 +186,12 @@ __device__ __forceinline__ int2 down_and_up(int field) {
     return make_int2(127 - e, 127 + e);
 }
 
+// fp16 numbers end at 2^-24, so the second one of a small decayed key would have few bits left: it is held times 2^11 (2^15 at most: the first is off by 16 at most), and
+// what it leaves out is 2^-22 of the key or 2^-36, which is 2^-22 of the smallest normal key.  The first launch sums up its products apart; in the second, where tensor
+// memory has no room for that, the state is held times 2^11 as well while they are added, and taken back by the MMA that adds the first product.
+constexpr int kSecondShift = 11;
+constexpr float kSecondTimes = 1 << kSecondShift;
+
 // A box of a tensor map into shared memory, from `row` and the first dim `x` on (a multiple of 64).
 __device__ __forceinline__ void prefetch_map(const CUtensorMap& map) { asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map)) : "memory"); }
 __device__ __forceinline__ void tma_load(unsigned char* dst, const CUtensorMap& map, int x, int row, uint64_t* bar) {
@@ -228,7 +234,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
     using Smem = LinearSmem<D>;
     // in the first launch the row warps help with the keys
     constexpr int kKeyWarps = kSums ? kLastWarps : kStateWarps, kKeyThreads = kKeyWarps * 32, kHalf = 4 * D / kKeyWarps;  // kHalf: columns of the state such a warp has
-    constexpr uint32_t kStateCol = 0, kOperandCol = D, kScoreCol = D + D / 2, kBeforeCol = kScoreCol + 2 * kC, kInsideCol = kBeforeCol + 2 * kC;
+    // kSecondCol: of the first launch in fp16, the products of the keys' second numbers
+    constexpr uint32_t kStateCol = 0, kSecondCol = kSums && !kBf16 ? D : 0, kOperandCol = D, kScoreCol = D + D / 2, kBeforeCol = kScoreCol + 2 * kC, kInsideCol = kBeforeCol + 2 * kC;
     static_assert(kInsideCol + kC <= kTmemCols, "tensor memory");
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
@@ -428,10 +435,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                 tc::fence_after_sync();
                 if (tc::elect_one()) {
                     const uint64_t a = dims_desc(st.v), b = keys_desc(st.k), b2 = keys_desc(sm.second[c & 1]);
+                    auto second = [&](int s, bool accumulate) { tc::mma_f16_ss(tmem + kStateCol + kSecondCol, tc::desc_at(a, s * 2048), tc::desc_at(b2, s * 2048), kState, accumulate); };
+                    auto first = [&](int s, bool accumulate) { tc::mma_f16_ss(tmem + kStateCol, tc::desc_at(a, s * 2048), tc::desc_at(b, s * 2048), kState, accumulate); };
+                    if constexpr (!kBf16 && !kSums) {
 #pragma unroll
-                    for (int s = 0; s < kC / 16; ++s) tc::mma_f16_ss(tmem + kStateCol, tc::desc_at(a, s * 2048), tc::desc_at(b, s * 2048), kState, !kSums || c > 0 || s > 0);
+                        for (int s = 0; s < kC / 16; ++s) second(s, true);
+                        tc::mma_f16_ss_scaled<kSecondShift>(tmem + kStateCol, a, b, kState);
 #pragma unroll
-                    for (int s = 0; s < kC / 16; ++s) tc::mma_f16_ss(tmem + kStateCol, tc::desc_at(a, s * 2048), tc::desc_at(b2, s * 2048), kState, true);
+                        for (int s = 1; s < kC / 16; ++s) first(s, true);
+                    } else {
+#pragma unroll
+                        for (int s = 0; s < kC / 16; ++s) first(s, !kSums || c > 0 || s > 0);
+#pragma unroll
+                        for (int s = 0; s < kC / 16; ++s) second(s, kBf16 || c > 0 || s > 0);
+                    }
                     if (!kSums) {
                         const uint64_t q = rows_desc(st.q);
 #pragma unroll
@@ -505,7 +522,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                     for (int e = 0; e < 4; ++e) {
                         const F2 x = mul2(pair_of<kBf16>(in[e]), F2(w, w));
                         a[e] = pack_pair<kBf16>(x);
-                        b[e] = zero_if_nan<kBf16>(pack_pair<kBf16>(sub2(x, pair_of<kBf16>(a[e]))));
+                        b[e] = zero_if_nan<kBf16>(pack_pair<kBf16>(mul2(sub2(x, pair_of<kBf16>(a[e])), F2(kSecondTimes, kSecondTimes))));
                     }
                 }
                 *reinterpret_cast<uint4*>(keys + 16 * u) = make_uint4(a[0], a[1], a[2], a[3]);
@@ -531,7 +548,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                 // the state as an operand, and decayed over the chunk
                 if (c > 0 && !wait3(sm.done, c - 1)) break;
                 tc::fence_after_sync();
-                const float decay = decay_power(g, min(kC, end - begin - c * kC));
+                const float decay = decay_power(g, min(kC, end - begin - c * kC)) * (kBf16 ? 1.0f : kSecondTimes);
                 float down = 1.0f;
                 if constexpr (!kBf16) {
                     float most = 0.0f;
@@ -590,6 +607,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(const __grid_co
                     for (int e = 0; e < 16; ++e) first[e] = from[e * D];
                 }
                 tc::tmem_ld16(state_at + b, r);
+                if constexpr (kSecondCol != 0) {
+                    uint32_t second[16];
+                    tc::tmem_ld16(state_at + kSecondCol + b, second);
+                    tc::tmem_ld_wait();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(fmaf(__uint_as_float(second[e]), 1.0f / kSecondTimes, __uint_as_float(r[e])));
+                }
                 tc::tmem_ld_wait();
                 if (row < D) {
 #pragma unroll

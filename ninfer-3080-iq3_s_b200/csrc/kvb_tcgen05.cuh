@@ -66,6 +66,16 @@ __device__ __forceinline__ void mma_f16_ss(uint32_t tmem_d, uint64_t desc_a, uin
         ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
         : "memory");
 }
+// D[tmem] = D[tmem] * 2^-kShift + A[smem] * B[smem], kShift 0 .. 15.
+template <int kShift> __device__ __forceinline__ void mma_f16_ss_scaled(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc) {
+    static_assert(kShift >= 0 && kShift <= 15, "scale of D");
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, 1, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p, %4;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "n"(kShift)
+        : "memory");
+}
 // D[tmem] (+)= A[tmem] * B[smem]: the A operand (M x 16, 16-bit elements) is read from tensor memory, lane = row,
 // two elements per 32-bit column (even k in the low half), 8 columns per instruction.
 __device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, bool accumulate) {
