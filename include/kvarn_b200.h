@@ -292,7 +292,8 @@ int kvb_rope_append(const kvb_layer* layer, const kvb_rope* rope, const void* q,
  * the keys.  For handing a prefix on, or comparing; the reference keeps such rows in its bf16 mirror (LAUNCH.h:70-91). */
 int kvb_read_rows(const kvb_layer* layer, int begin, int tokens, const int32_t* total_pos_dev, void* out_k, void* out_v, void* stream);
 
-/* ---- Linear attention with a decay for each head: the layers of a hybrid model that keep a state instead of a cache.  No counterpart in the reference. ----
+/* ---- Linear attention with one decay for each head, the same at every token: layers of a hybrid model that keep a state instead of a cache.  No
+ * counterpart in the reference. ----
  *   S_t = exp(log_decay[head]) S_{t-1} + k_t v_t^T,   o_t = scale * q_t S_t
  * per sequence and value head; S: [head_dim of k][head_dim of v], fp32.  Value head h goes with query and key head h / (v_heads / qk_heads). */
 typedef struct kvb_linear {
@@ -318,7 +319,9 @@ int kvb_linear_decode(const kvb_linear* layer, const void* q, int64_t q_stride, 
  * b (offsets_dev[batch + 1], not falling, within 0..tokens; a sequence without rows has its state copied).  Rows outside all sequences are left as they are.
  * Offsets that fall or leave the rows set KVB_ERR_POSITIONS; that sequence is left alone.  Where offsets that fall make sequences share rows, an output is
  * that of one of them, and a sequence may be left alone for want of places in the workspace (KVB_ERR_POSITIONS).
- * An infinite key leaves the recurrence's infinities; an infinite value may leave NaN in its column of the state, as may a decay that rounds to 0 on the way.
+ * How a call is cut goes by the mean length: single tokens beside long prompts are better off in a kvb_linear_decode of their own.
+ * An infinite key leaves the recurrence's infinities; an infinite value may leave NaN in its column of the state, as may a decay that rounds to 0 on the
+ * way.  With rows of fp16, states go to 2^116.
  * workspace: kvb_linear_workspace_bytes(tokens, batch, ...) bytes, not shared by calls that overlap on the GPU. */
 size_t kvb_linear_workspace_bytes(int tokens, int batch, int v_heads, int head_dim);
 int kvb_linear_chunk(const kvb_linear* layer, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,

@@ -10,8 +10,8 @@
 // chunk to chunk, and is an A operand there too; only rows of tokens as they come from global memory, decayed keys and P lie in shared memory.
 // Roundings: P, and the state as an operand, to the type, like the output that they are summed up to (both together as much as the output's own
 // rounding); decayed keys as two numbers of the type, whose sum has 16 bits of bf16 or 22 of fp16 (2^-36 where these are less), so that states keep their
-// precision over long prompts: 4e-6 of the state's norm in bf16 (a third number would take 32 KB of shared memory that are not there), 2e-7 in fp16.  Heads of 64 dims fill both halves
-// of the M rows with the same 64; the scores' 64 rows are the first of 128, and what the others multiply is not looked at.
+// precision over long prompts: 4e-6 of the state's norm in bf16 (a third number would take 32 KB of shared memory that are not there), 5e-7 in fp16.
+// Heads of 64 dims fill both halves of the M rows with the same 64; the scores' 64 rows are the first of 128, and what the others multiply is not looked at.
 //
 // Warps by role, so that a chunk's steps run beside its neighbours':
 //   state warps   the state as an operand (then decayed over the chunk), decayed keys of the next chunk
@@ -30,8 +30,8 @@
 //
 // Bound by the hand-overs between warps and tensor cores: two loops of about 3,800 cycles a chunk, in which no role's own work is more than an eighth
 // (left out one at a time, none shortens a chunk by more than 13 %); the tensor pipe is busy for 22 % of the time, memory for 26.  Measured on B200,
-// graph replay: 8,192 tokens of 32 value heads of 128 dims 108 us (floor 31), 1.9 TB/s of q, k, v, o once; 7 prompts of 9,001 tokens, 24 heads
-// of 64 dims 66 us with states of 32 KB a head (floor 18); 300 tokens 18 us.  Chunks of 128 tokens, whose products do a half more for the same rows,
+// graph replay, bf16 / fp16: 8,192 tokens of 32 value heads of 128 dims 110 / 138 us (floor 31), 1.9 TB/s of q, k, v, o once; 7 prompts of 9,001 tokens, 24 heads
+// of 64 dims 52 / 66 us with states of 16 KB a head (floor 18); 300 tokens 18 / 22 us.  Chunks of 128 tokens, whose products do a half more for the same rows,
 // were slower (2,048 tokens of 128 heads 89 ... 106 us, of 64 tokens 77), so were outputs stored by TMA (90).
 //
 // In fp16 the scores of a row and the state's rows are scaled by a power of two to a largest magnitude of 2^14 .. 2^15 before they are rounded, so that

@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(LayerView L, int beg
                     auto rotated = [&](int s, F2 (&x)[8][2][2]) {  // slice s of 16 tokens: [group][j][token g, token g + 8], times what belongs to the token
                         const float a0 = sm.token_a[s][row0], a1 = sm.token_a[s][row1], b0 = sm.token_b[s][row0], b1 = sm.token_b[s][row1];
                         uint32_t w[2][4];
-        #pragma unroll
+#pragma unroll
                         for (int side = 0; side < 2; ++side) {
                             const uint2 r0 = *reinterpret_cast<const uint2*>(code + row0 * G::kCodeLeading + 64 * s + 32 * side + 8 * t);
                             const uint2 r1 = *reinterpret_cast<const uint2*>(code + row1 * G::kCodeLeading + 64 * s + 32 * side + 8 * t);
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(LayerView L, int beg
                             w[1][2 * side] = r1.x;
                             w[1][2 * side + 1] = r1.y;
                         }
-        #pragma unroll
+#pragma unroll
                         for (int group = 0; group < 8; ++group) {
                             uint32_t a[4];
                             if constexpr (kCodes) {
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(LayerView L, int beg
                             }
                             const uint2 b = signed_dims(sm.dim_a[s][0], group);
                             const float4 term = *reinterpret_cast<const float4*>(&sm.term[s][t][4 * group]);
-        #pragma unroll
+#pragma unroll
                             for (int j = 0; j < 2; ++j) {
                                 const float t0 = j ? term.z : term.x, t1 = j ? term.w : term.y;
                                 float d[4];
@@ -269,15 +269,15 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(LayerView L, int beg
                         rotate_groups(x);
                     };
                     auto store = [&](int s, const F2 (&x)[8][2][2]) {
-        #pragma unroll
+#pragma unroll
                         for (int half = 0; half < 2; ++half) {
                             const int at = tile * kTile + (half ? row1 : row0);
                             if (at < rows.x || at > rows.y) continue;
                             uint16_t* const to = out + (static_cast<int64_t>(at - begin) * L.kv_heads + head) * D + 128 * s + 16 * t;
-        #pragma unroll
+#pragma unroll
                             for (int side = 0; side < 2; ++side) {
                                 uint32_t o[8];
-        #pragma unroll
+#pragma unroll
                                 for (int e = 0; e < 8; ++e) {
                                     const float2 y = x[4 * side + (e >> 1)][e & 1][half].get();
                                     o[e] = pack_out<kBf16>(y);
@@ -298,11 +298,11 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(LayerView L, int beg
                     } else {
                         F2 y[8][2][2];
                         rotated(1, y);
-        #pragma unroll
+#pragma unroll
                         for (int group = 0; group < 8; ++group)
-        #pragma unroll
+#pragma unroll
                             for (int j = 0; j < 2; ++j)
-        #pragma unroll
+#pragma unroll
                                 for (int r = 0; r < 2; ++r) {
                                     const F2 lo = x[group][j][r], hi = y[group][j][r];
                                     x[group][j][r] = add2(lo, hi);

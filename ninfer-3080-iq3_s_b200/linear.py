@@ -1,4 +1,4 @@
-"""Linear attention with a decay for each head: the layers of a hybrid model that keep a state per sequence instead of a cache."""
+"""Linear attention with one decay for each head, the same at every token: layers of a hybrid model that keep a state per sequence instead of a cache."""
 from __future__ import annotations
 
 import ctypes as C
